@@ -292,6 +292,64 @@ size_t krea2_quantized_static_workspace_bytes(void);
 int krea2_quantized_forward_static(krea2_stream stream, size_t rows, const void *x, const void *weight,
                                    const float *scales, void *out, size_t inputs, size_t outputs);
 
+/* ---------------------------------------------------------------- e4m3 projections, rotary positions, cross attention
+ * New with this library: a cross-attention sublayer beside the W8A8 block.  Tensors are f16 or bf16 as `kind` says;
+ * strides are elements from one row to the next and everything inside a row is contiguous.  The stream and the
+ * buffers belong to the device that is current in the calling thread.  Nothing here keeps a workspace or any state
+ * between calls: any number of them, captured or not, may overlap. */
+enum { KREA2_F16 = 0, KREA2_BF16 = 1 };
+
+/* Codes q e4m3 [tokens][out_stride] with one scale per 128 channels, q_scale f32 [tokens][ceil(width/128)]:
+ * scale = max(max|y| / 448, 2^-126), code = e4m3(y * (1/scale)) to nearest even.  y is the row x itself, or
+ * x / sqrt(mean(x^2) + eps) * (weight_offset + weight[i]) where x has first become kind(x + residual) if there is a
+ * residual (`sum`, if not NULL, receives it: it may be the buffer of x or of residual).  weight f32 [width] or NULL for
+ * zeros; weight_offset 1 suits weights stored minus one, as this library's checkpoints hold them, 0 plain ones.  A NaN
+ * stays a NaN code in its place; an infinity makes its group (after a norm: its place) NaN.  width 1..32768, out_stride
+ * a multiple of 16. */
+int krea2_prepare_norm_fp8(krea2_stream stream, size_t tokens, const void *x, const void *residual, const float *weight,
+                           void *sum, void *q, float *q_scale, size_t width, size_t x_stride, size_t residual_stride,
+                           size_t sum_stride, size_t out_stride, float eps, float weight_offset, int kind);
+int krea2_prepare_plain_fp8(krea2_stream stream, size_t tokens, const void *x, void *q, float *q_scale, size_t width,
+                            size_t x_stride, size_t out_stride, int kind);
+
+/* c[i][j] = kind(sum over blocks g of 128 channels: a_scale[i][g] * scale[j/128][g] * sum of a[i][k] * w[j][k] in g).
+ * a e4m3 [m][a_stride], w e4m3 [n_size][w_stride], both K-contiguous; a_scale f32 [m][ceil(k_size/128)], scale f32
+ * [ceil(n_size/128)][ceil(k_size/128)].  Any m, n_size and k_size (up to 2^24, 262144, 65536); a_stride and w_stride
+ * multiples of 16, codes beyond k_size are never used. */
+int krea2_gemm_fp8_128(krea2_stream stream, size_t m, const void *a, const void *w, const float *scale,
+                       const float *a_scale, void *c, size_t k_size, size_t a_stride, size_t w_stride, size_t n_size,
+                       size_t c_stride, int kind);
+
+/* Rotary positions: pair i of a head, channels (2i, 2i+1) or (i, i + rotary_dim/2), is turned by positions[token] *
+ * frequencies[i] radians and multiplied by `magnitude`; channels from rotary_dim on are copied.  inverse = 1 turns
+ * back: the gradient of the inputs from the gradient of the outputs.  q [tokens][q_heads*head_dim], k
+ * [tokens][kv_heads*head_dim] (kv_heads 0 and NULL for none), in place where the outputs are the inputs; positions
+ * int32 [tokens] or NULL for the row numbers; frequencies f64 [rotary_dim/2].  head_dim 2..512. */
+enum { KREA2_ROTARY_INTERLEAVED = 0, KREA2_ROTARY_HALF = 1 };
+int krea2_rotary(krea2_stream stream, size_t tokens, const void *q, const void *k, const int32_t *positions,
+                 const double *frequencies, void *q_out, void *k_out, size_t q_heads, size_t kv_heads, size_t head_dim,
+                 size_t rotary_dim, size_t q_stride, size_t k_stride, size_t q_out_stride, size_t k_out_stride,
+                 float magnitude, int layout, int inverse, int kind);
+/* The frequencies base^(-2i/rotary_dim), i < rotary_dim/2, and the magnitude 1 (host work, no device is touched).  For
+ * contexts `factor` times the `trained` length: LINEAR divides all by factor; BASE raises the base so that the slowest
+ * is divided by factor and the fastest kept; PARTS keeps those that turn `fast` times or more within `trained`
+ * positions, divides those that turn `slow` times or less, blends between, and takes the magnitude 0.1 ln(factor) + 1. */
+enum { KREA2_ROTARY_PLAIN = 0, KREA2_ROTARY_LINEAR = 1, KREA2_ROTARY_BASE = 2, KREA2_ROTARY_PARTS = 3 };
+int krea2_rotary_frequencies(size_t rotary_dim, double base, int scaling, double factor, double trained, double slow,
+                             double fast, double *host_frequencies, float *host_magnitude);
+
+/* out[b][i][h] = softmax over keys j of scale * (q[b][i][h] . k[b][j][h']) applied to v[b][j][h'], h' = h / (q_heads /
+ * kv_heads).  A key counts if j < kv_lengths[b] (int32 [batch], clamped to 0..kv_len; NULL: kv_len) and key_mask
+ * (bytes [batch][mask_stride]; NULL: all) is not zero there; whatever lies in keys and values that do not count, NaN
+ * included, changes nothing, and a row without a counting key is written as zeros.  q, out [batch][q_len][q_heads *
+ * head_dim], k, v [batch][kv_len][kv_heads * head_dim] at 16-byte aligned rows (strides multiples of 8); head_dim a
+ * multiple of 8 up to 128; kv_len may be 0; scale > 0. */
+int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q_len, size_t kv_len, const void *q, const void *k,
+                          const void *v, const int32_t *kv_lengths, const void *key_mask, void *out, size_t q_heads,
+                          size_t kv_heads, size_t head_dim, size_t q_batch_stride, size_t q_stride,
+                          size_t k_batch_stride, size_t k_stride, size_t v_batch_stride, size_t v_stride,
+                          size_t out_batch_stride, size_t out_stride, size_t mask_stride, float scale, int kind);
+
 /* ---------------------------------------------------------------- generic dispatch
  * Ops::launch (src/ops/mod.rs:673-693): kernel by stem, config keys by name, packed
  * scalars, buffers in binding order, and the launch geometry the reference would use

@@ -8,6 +8,7 @@ use std::path::PathBuf;
 
 const SOURCES: &[&str] = &[
     "api.cu", "prepare.cu", "gemm_i8.cu", "session.cu", "quantized.cu", "attention.cu", "sampler.cu", "checkpoint.cu",
+    "fp8.cu", "rotary.cu", "cross_attention.cu",
 ];
 
 fn main() {

@@ -32,6 +32,15 @@ pub const KREA2_SHARD_PLAIN: c_int = 0;
 pub const KREA2_SHARD_RESID: c_int = 1;
 pub const KREA2_SHARD_SWIGLU: c_int = 2;
 
+pub const KREA2_F16: c_int = 0;
+pub const KREA2_BF16: c_int = 1;
+pub const KREA2_ROTARY_INTERLEAVED: c_int = 0;
+pub const KREA2_ROTARY_HALF: c_int = 1;
+pub const KREA2_ROTARY_PLAIN: c_int = 0;
+pub const KREA2_ROTARY_LINEAR: c_int = 1;
+pub const KREA2_ROTARY_BASE: c_int = 2;
+pub const KREA2_ROTARY_PARTS: c_int = 3;
+
 /// One `config` key of a name-keyed launch (`Ops::launch`, src/ops/mod.rs:673-693).
 #[repr(C)]
 pub struct krea2_config_entry {
@@ -147,6 +156,12 @@ extern "C" {
     pub fn krea2_quantized_forward(stream: krea2_stream, rows: usize, x: *const c_void, weight: *const c_void, scales: *const f32, out: *mut c_void, inputs: usize, outputs: usize, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn krea2_quantized_static_workspace_bytes() -> usize;
     pub fn krea2_quantized_forward_static(stream: krea2_stream, rows: usize, x: *const c_void, weight: *const c_void, scales: *const f32, out: *mut c_void, inputs: usize, outputs: usize) -> c_int;
+    pub fn krea2_prepare_norm_fp8(stream: krea2_stream, tokens: usize, x: *const c_void, residual: *const c_void, weight: *const f32, sum: *mut c_void, q: *mut c_void, q_scale: *mut f32, width: usize, x_stride: usize, residual_stride: usize, sum_stride: usize, out_stride: usize, eps: f32, weight_offset: f32, kind: c_int) -> c_int;
+    pub fn krea2_prepare_plain_fp8(stream: krea2_stream, tokens: usize, x: *const c_void, q: *mut c_void, q_scale: *mut f32, width: usize, x_stride: usize, out_stride: usize, kind: c_int) -> c_int;
+    pub fn krea2_gemm_fp8_128(stream: krea2_stream, m: usize, a: *const c_void, w: *const c_void, scale: *const f32, a_scale: *const f32, c: *mut c_void, k_size: usize, a_stride: usize, w_stride: usize, n_size: usize, c_stride: usize, kind: c_int) -> c_int;
+    pub fn krea2_rotary(stream: krea2_stream, tokens: usize, q: *const c_void, k: *const c_void, positions: *const i32, frequencies: *const f64, q_out: *mut c_void, k_out: *mut c_void, q_heads: usize, kv_heads: usize, head_dim: usize, rotary_dim: usize, q_stride: usize, k_stride: usize, q_out_stride: usize, k_out_stride: usize, magnitude: f32, layout: c_int, inverse: c_int, kind: c_int) -> c_int;
+    pub fn krea2_rotary_frequencies(rotary_dim: usize, base: f64, scaling: c_int, factor: f64, trained: f64, slow: f64, fast: f64, host_frequencies: *mut f64, host_magnitude: *mut f32) -> c_int;
+    pub fn krea2_cross_attention(stream: krea2_stream, batch: usize, q_len: usize, kv_len: usize, q: *const c_void, k: *const c_void, v: *const c_void, kv_lengths: *const i32, key_mask: *const c_void, out: *mut c_void, q_heads: usize, kv_heads: usize, head_dim: usize, q_batch_stride: usize, q_stride: usize, k_batch_stride: usize, k_stride: usize, v_batch_stride: usize, v_stride: usize, out_batch_stride: usize, out_stride: usize, mask_stride: usize, scale: f32, kind: c_int) -> c_int;
     pub fn krea2_launch(stream: krea2_stream, name: *const c_char, config: *const krea2_config_entry, config_count: usize, indices: *const u64, index_count: usize, bindings: *const krea2_binding, binding_count: usize, grid_x: usize, grid_y: usize, threads: u32) -> c_int;
     pub fn krea2_shape_tokens_min() -> usize;
     pub fn krea2_shape_tokens_max() -> usize;

@@ -122,6 +122,21 @@ SIGNATURES = {
     "krea2_quantized_static_workspace_bytes": (c_size_t, []),
     "krea2_quantized_forward_static": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                                c_size_t]),
+    "krea2_prepare_norm_fp8": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_float, c_float,
+                                       c_int]),
+    "krea2_prepare_plain_fp8": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t,
+                                        c_size_t, c_int]),
+    "krea2_gemm_fp8_128": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_size_t, c_size_t, c_size_t, c_size_t, c_int]),
+    "krea2_rotary": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_float,
+                             c_int, c_int, c_int]),
+    "krea2_rotary_frequencies": (c_int, [c_size_t, c_double, c_int, c_double, c_double, c_double, c_double, c_void_p,
+                                         c_void_p]),
+    "krea2_cross_attention": (c_int, [c_void_p, c_size_t, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t,
+                                      c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_float, c_int]),
     "krea2_launch": (c_int, [c_void_p, c_char_p, POINTER(ConfigEntry), c_size_t, POINTER(c_uint64), c_size_t,
                              POINTER(Binding), c_size_t, c_size_t, c_size_t, c_uint32]),
     "krea2_shape_tokens_min": (c_size_t, []),

@@ -87,6 +87,16 @@ __device__ __forceinline__ float bf_round(float x) { return __bfloat162float(__f
 // f32 -> f16 -> f32, IEEE round to nearest even.
 __device__ __forceinline__ float hf_round(float x) { return __half2float(__float2half_rn(x)); }
 
+// A bf16 or f16 pattern as f32, and back with one rounding to nearest even.
+template <bool kBf16>
+__device__ __forceinline__ float value_of(uint16_t bits) {
+    return kBf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
+}
+template <bool kBf16>
+__device__ __forceinline__ uint16_t bits_of(float v) {
+    return kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+
 // exp with a fixed evaluation order: Cody-Waite reduction by ln 2 in two pieces, the degree-6
 // Cephes polynomial, scaling by two exact powers of two.  It stands in for the reference's
 // approximate `expf<afn>` (kernels/prepare_gated_i8.loom:99, gemm_i8_swiglu_256.loom:650).

@@ -250,3 +250,219 @@ def guidance(cond, uncond, scale, stream=None):
     if tuple(cond.shape) != tuple(uncond.shape):
         raise InvalidArgument("guidance tensor dimensions")
     check(lib().krea2_guidance(_stream_ptr(stream), cond.numel(), float(scale), _ptr(cond), _ptr(uncond)))
+
+
+# ------------------------------------------------------------------ e4m3 projections, rotary positions, cross attention
+# New with this library.  Rows may have any pitch the C ABI takes (a slice of a wider tensor is fine); a call runs on the
+# tensors' device, on `stream` or that device's current stream.
+KINDS = {torch.float16: 0, torch.bfloat16: 1}
+GROUP = 128  # channels under one scale
+ROTARY_LAYOUTS = {"interleaved": 0, "half": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+def _groups(width: int) -> int:
+    return -(-width // GROUP)
+
+
+def _kind(name, t: torch.Tensor) -> int:
+    kind = KINDS.get(t.dtype)
+    if kind is None:
+        raise InvalidArgument(f"{name}: {t.dtype} is neither float16 nor bfloat16")
+    return kind
+
+
+def _check_rows(name, what, t, shape, dtype, device, lead=1) -> None:
+    """A tensor of that shape and type on that device whose dimensions after the first `lead` lie in one piece."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise InvalidArgument(f"{name}: {what} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    if t.device != device or not t.is_cuda:
+        raise InvalidArgument(f"{name}: {what} is on {t.device}: buffers must share one CUDA device")
+    if not t.is_contiguous():
+        inner, strides = 1, t.stride()
+        for i in range(len(shape) - 1, lead - 1, -1):
+            if shape[i] != 1 and strides[i] != inner:
+                raise InvalidArgument(f"{name}: the rows of {what} must be contiguous")
+            inner *= shape[i]
+
+
+def _row_stride(t: torch.Tensor, inner: int) -> int:
+    """Elements from one row to the next; a lone row's stride carries no meaning."""
+    return t.stride(0) if t.shape[0] > 1 else inner
+
+
+def _padded(stride: int) -> int:
+    return -(-stride // 16) * 16
+
+
+def _run_on(name, device: torch.device, stream, fn, *args) -> None:
+    if stream is not None and stream.device != device:
+        raise InvalidArgument(f"{name}: the stream belongs to {stream.device}, the buffers to {device}")
+    if device.index == torch.cuda.current_device():
+        check(fn((stream or torch.cuda.current_stream()).cuda_stream, *args))
+    else:
+        with torch.cuda.device(device):
+            check(fn((stream or torch.cuda.current_stream()).cuda_stream, *args))
+
+
+def prepare_norm_fp8(x, weight, q, q_scale, residual=None, sum_out=None, eps=1e-5, weight_offset=0.0, stream=None):
+    """RMS norm of x [tokens][width] (after x + residual, which `sum_out` receives, if there is one) times
+    (weight_offset + weight), as e4m3 codes q with q_scale f32 [tokens][ceil(width/128)]."""
+    name, device, (tokens, width) = "prepare_norm_fp8", x.device, x.shape
+    kind = _kind(name, x)
+    _check_rows(name, "x", x, (tokens, width), x.dtype, device)
+    _check_rows(name, "q", q, (tokens, width), torch.float8_e4m3fn, device)
+    _check_rows(name, "q_scale", q_scale, (tokens, _groups(width)), torch.float32, device)
+    for what, t in (("residual", residual), ("sum_out", sum_out)):
+        if t is not None:
+            _check_rows(name, what, t, (tokens, width), x.dtype, device)
+    if weight is not None and (weight.dtype != torch.float32 or weight.numel() != width or weight.device != device):
+        raise InvalidArgument(f"{name}: weight must be float32 [{width}] on {device}")
+    _run_on(name, device, stream, lib().krea2_prepare_norm_fp8, tokens, x.data_ptr(), residual.data_ptr() if residual is not None else None,
+            _ptr(weight) if weight is not None else None, sum_out.data_ptr() if sum_out is not None else None, q.data_ptr(), _ptr(q_scale),
+            width, _row_stride(x, width), _row_stride(residual, width) if residual is not None else 0,
+            _row_stride(sum_out, width) if sum_out is not None else 0, _row_stride(q, _padded(width)), eps, weight_offset, kind)
+
+
+def prepare_plain_fp8(x, q, q_scale, stream=None):
+    """e4m3 codes of x [tokens][width] with one scale per 128 channels (prepare_norm_fp8 without the norm)."""
+    name, device, (tokens, width) = "prepare_plain_fp8", x.device, x.shape
+    kind = _kind(name, x)
+    _check_rows(name, "x", x, (tokens, width), x.dtype, device)
+    _check_rows(name, "q", q, (tokens, width), torch.float8_e4m3fn, device)
+    _check_rows(name, "q_scale", q_scale, (tokens, _groups(width)), torch.float32, device)
+    _run_on(name, device, stream, lib().krea2_prepare_plain_fp8, tokens, x.data_ptr(), q.data_ptr(), _ptr(q_scale), width,
+            _row_stride(x, width), _row_stride(q, _padded(width)), kind)
+
+
+def gemm_fp8_128(a, a_scale, w, w_scale, c, stream=None):
+    """c [m][n] (f16 or bf16) = a [m][k] times w [n][k] transposed, e4m3 codes under a_scale f32 [m][ceil(k/128)] and
+    w_scale f32 [ceil(n/128)][ceil(k/128)]."""
+    name, device, (m, k), n = "gemm_fp8_128", a.device, a.shape, w.shape[0]
+    kind = _kind(name, c)
+    _check_rows(name, "a", a, (m, k), torch.float8_e4m3fn, device)
+    _check_rows(name, "w", w, (n, k), torch.float8_e4m3fn, device)
+    _check_rows(name, "a_scale", a_scale, (m, _groups(k)), torch.float32, device)
+    _check_rows(name, "w_scale", w_scale, (_groups(n), _groups(k)), torch.float32, device)
+    _check_rows(name, "c", c, (m, n), c.dtype, device)
+    _run_on(name, device, stream, lib().krea2_gemm_fp8_128, m, a.data_ptr(), w.data_ptr(), _ptr(w_scale), _ptr(a_scale), c.data_ptr(), k,
+            _row_stride(a, _padded(k)), _row_stride(w, _padded(k)), n, _row_stride(c, n), kind)
+
+
+class QuantizedFp8:
+    """One projection on f16 or bf16 rows through e4m3 codes (the e4m3 sibling of Quantized): prepare_plain_fp8, or
+    prepare_norm_fp8 where a norm precedes it, then gemm_fp8_128."""
+
+    def __init__(self, weight: torch.Tensor):
+        """`weight` [outputs][inputs] in a floating type on the device that the calls will run on; kept as e4m3 codes with
+        one scale per 128 x 128 block."""
+        if weight.dim() != 2 or not weight.is_floating_point() or not weight.is_cuda or 0 in weight.shape:
+            raise InvalidArgument("an e4m3 projection takes a floating CUDA weight [outputs][inputs]")
+        self.outputs, self.inputs = weight.shape
+        rows, columns = _groups(self.outputs), _groups(self.inputs)
+        blocks = torch.zeros((rows * GROUP, columns * GROUP), dtype=torch.float32, device=weight.device)
+        blocks[: self.outputs, : self.inputs] = weight
+        blocks = blocks.view(rows, GROUP, columns, GROUP)
+        self.scales = (blocks.abs().amax((1, 3)) / 448.0).clamp_min_(2.0 ** -126)
+        codes = (blocks / self.scales[:, None, :, None]).clamp_(-448.0, 448.0).view(rows * GROUP, columns * GROUP)
+        pitch = _padded(self.inputs)
+        codes = codes[: self.outputs, : pitch].to(torch.float8_e4m3fn).view(torch.uint8).contiguous()
+        self.weight = codes.view(torch.float8_e4m3fn)[:, : self.inputs]
+
+    def buffers(self, rows: int):
+        """Codes and scales of `rows` input rows, for a caller that keeps them between calls."""
+        device = self.weight.device
+        q = torch.empty((rows, _padded(self.inputs)), dtype=torch.float8_e4m3fn, device=device)[:, : self.inputs]
+        return q, torch.empty((rows, _groups(self.inputs)), dtype=torch.float32, device=device)
+
+    def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, buffers=None, stream=None) -> torch.Tensor:
+        """x [rows][inputs] -> [rows][outputs] in x's type."""
+        return self._forward(x, out, buffers, stream, lambda q, s: prepare_plain_fp8(x, q, s, stream=stream))
+
+    def forward_norm(self, x: torch.Tensor, norm_weight: Optional[torch.Tensor], residual: Optional[torch.Tensor] = None,
+                     sum_out: Optional[torch.Tensor] = None, eps: float = 1e-5, weight_offset: float = 0.0,
+                     out: Optional[torch.Tensor] = None, buffers=None, stream=None) -> torch.Tensor:
+        """The projection of the RMS norm of x (+ residual, whose sum `sum_out` receives)."""
+        return self._forward(x, out, buffers, stream, lambda q, s: prepare_norm_fp8(
+            x, norm_weight, q, s, residual=residual, sum_out=sum_out, eps=eps, weight_offset=weight_offset, stream=stream))
+
+    def _forward(self, x, out, buffers, stream, prepare):
+        if x.dim() != 2 or x.shape[1] != self.inputs:
+            raise InvalidArgument("e4m3 projection dimensions")
+        # What is not given is allocated on the stream that uses it, so that the allocator reuses it in that stream's order.
+        with torch.cuda.stream(stream):
+            q, scale = buffers or self.buffers(x.shape[0])
+            if out is None:
+                out = torch.empty((x.shape[0], self.outputs), dtype=x.dtype, device=x.device)
+        prepare(q, scale)
+        gemm_fp8_128(q, scale, self.weight, self.scales, out, stream=stream)
+        return out
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling="none", factor=1.0, trained=0.0, slow=1.0, fast=32.0, device=None):
+    """(frequencies f64 [rotary_dim / 2] on `device`, magnitude) for ops.rotary; `scaling` "none", "linear", "base" or
+    "parts" for contexts `factor` times the `trained` length."""
+    if scaling not in ROTARY_SCALINGS:
+        raise InvalidArgument(f"rotary_frequencies: scaling is one of {', '.join(ROTARY_SCALINGS)}")
+    out = torch.empty(max(0, int(rotary_dim)) // 2, dtype=torch.float64)
+    magnitude = ctypes.c_float()
+    check(lib().krea2_rotary_frequencies(max(0, int(rotary_dim)), base, ROTARY_SCALINGS[scaling], factor, trained, slow, fast, out.data_ptr(),
+                                         ctypes.byref(magnitude)))
+    return out.to(device or "cuda"), magnitude.value
+
+
+def rotary(q, k, q_out, k_out, frequencies, positions=None, magnitude=1.0, layout="interleaved", inverse=False, stream=None):
+    """Turns q [tokens][q_heads][head_dim] and k [tokens][kv_heads][head_dim] (or None) by positions * frequencies into
+    q_out and k_out, which may be q and k; the first 2 * len(frequencies) channels of a head take part.  inverse=True is
+    the gradient's way back."""
+    name, device, (tokens, q_heads, head_dim) = "rotary", q.device, q.shape
+    kind, kv_heads = _kind(name, q), 0
+    for what, t in (("q", q), ("q_out", q_out)):
+        _check_rows(name, what, t, (tokens, q_heads, head_dim), q.dtype, device)
+    if (k is None) != (k_out is None):
+        raise InvalidArgument(f"{name}: k and k_out go together")
+    if k is not None:
+        kv_heads = k.shape[1]
+        for what, t in (("k", k), ("k_out", k_out)):
+            _check_rows(name, what, t, (tokens, kv_heads, head_dim), q.dtype, device)
+    if layout not in ROTARY_LAYOUTS:
+        raise InvalidArgument(f"{name}: layout is one of {', '.join(ROTARY_LAYOUTS)}")
+    if frequencies.dtype != torch.float64 or frequencies.device != device:
+        raise InvalidArgument(f"{name}: frequencies must be float64 on {device}")
+    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != tokens or positions.device != device):
+        raise InvalidArgument(f"{name}: positions must be int32 [{tokens}] on {device}")
+    q_row, k_row = q_heads * head_dim, kv_heads * head_dim
+    _run_on(name, device, stream, lib().krea2_rotary, tokens, q.data_ptr(), k.data_ptr() if kv_heads else None,
+            _ptr(positions) if positions is not None else None, _ptr(frequencies), q_out.data_ptr(), k_out.data_ptr() if kv_heads else None,
+            q_heads, kv_heads, head_dim, 2 * frequencies.numel(), _row_stride(q, q_row), _row_stride(k, k_row) if kv_heads else 0,
+            _row_stride(q_out, q_row), _row_stride(k_out, k_row) if kv_heads else 0, magnitude, ROTARY_LAYOUTS[layout], int(bool(inverse)), kind)
+
+
+def cross_attention(q, k, v, out, kv_lengths=None, key_mask=None, scale=None, stream=None):
+    """Attention of q [batch][q_len][q_heads][head_dim] to an encoder's k, v [batch][kv_len][kv_heads][head_dim], written
+    to `out` (shaped like q).  kv_lengths int32 [batch] and key_mask bool or uint8 [batch][kv_len] say which keys count
+    (both: those that both name); a query without one gets zeros.  scale defaults to head_dim ** -0.5."""
+    name, device, (batch, q_len, q_heads, head_dim) = "cross_attention", q.device, q.shape
+    kind, kv_len, kv_heads = _kind(name, q), k.shape[1], k.shape[2]
+    for what, t in (("q", q), ("out", out)):
+        _check_rows(name, what, t, (batch, q_len, q_heads, head_dim), q.dtype, device, 2)
+    for what, t in (("k", k), ("v", v)):
+        _check_rows(name, what, t, (batch, kv_len, kv_heads, head_dim), q.dtype, device, 2)
+    if kv_lengths is not None and (kv_lengths.dtype != torch.int32 or kv_lengths.numel() != batch or kv_lengths.device != device):
+        raise InvalidArgument(f"{name}: kv_lengths must be int32 [{batch}] on {device}")
+    mask_stride = 0
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8):
+            raise InvalidArgument(f"{name}: key_mask must be bool or uint8")
+        _check_rows(name, "key_mask", key_mask, (batch, kv_len), key_mask.dtype, device)
+        mask_stride = _row_stride(key_mask, kv_len)
+    q_row, k_row = q_heads * head_dim, kv_heads * head_dim
+
+    def strides(t, row):
+        rows = t.stride(1) if t.shape[1] > 1 else row
+        return (t.stride(0) if batch > 1 else t.shape[1] * rows), rows
+
+    _run_on(name, device, stream, lib().krea2_cross_attention, batch, q_len, kv_len, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _ptr(kv_lengths) if kv_lengths is not None else None, key_mask.data_ptr() if key_mask is not None else None, out.data_ptr(),
+            q_heads, kv_heads, head_dim, *strides(q, q_row), *strides(k, k_row), *strides(v, k_row), *strides(out, q_row), mask_stride,
+            head_dim ** -0.5 if scale is None else scale, kind)
