@@ -8,7 +8,7 @@ use std::path::PathBuf;
 
 const SOURCES: &[&str] = &[
     "api.cu", "prepare.cu", "gemm_i8.cu", "session.cu", "quantized.cu", "attention.cu", "sampler.cu", "checkpoint.cu",
-    "fp8.cu", "rotary.cu", "cross_attention.cu",
+    "prepare_fp8.cu", "gemm_fp8.cu", "rotary.cu", "cross_attention.cu",
 ];
 
 fn main() {
@@ -31,6 +31,7 @@ fn main() {
         build.file(path);
     }
     println!("cargo:rerun-if-changed={}", csrc.join("common.cuh").display());
+    println!("cargo:rerun-if-changed={}", csrc.join("tensor_core.cuh").display());
     println!("cargo:rerun-if-changed={}", root.join("include").join("krea2_b200.h").display());
     build.compile("krea2_b200");
     println!("cargo:rustc-link-lib=cudart");

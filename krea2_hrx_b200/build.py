@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkrea2_b200.so")
 SOURCES = ["api.cu", "prepare.cu", "gemm_i8.cu", "session.cu", "quantized.cu", "attention.cu", "sampler.cu", "checkpoint.cu",
-           "fp8.cu", "rotary.cu", "cross_attention.cu"]
+           "prepare_fp8.cu", "gemm_fp8.cu", "rotary.cu", "cross_attention.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-O2,-Wall", "--expt-relaxed-constexpr",

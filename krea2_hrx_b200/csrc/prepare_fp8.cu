@@ -1,7 +1,6 @@
-// Projections in e4m3 with one scale per 128 channels (new with this library; the reference's projections are int8):
+// Activations as e4m3 codes with one scale per 128 channels (new with this library; the reference's projections are int8):
 //   krea2_prepare_norm_fp8   the residual's addition, the RMS norm and the codes of its result in one pass
 //   krea2_prepare_plain_fp8  the codes of rows as they are
-//   krea2_gemm_fp8_128       the product of two code matrices under their block scales
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -171,45 +170,6 @@ int check_prepare(const char *name, size_t tokens, const void *x, const void *q,
     return KREA2_OK;
 }
 
-// ---------------------------------------------------------------- product
-struct ProductArgs {
-    const uint8_t *a, *w;
-    const float *w_scale, *a_scale;
-    uint16_t *c;
-    uint32_t m, n, k, k_groups;
-    size_t a_stride, w_stride, c_stride;
-};
-
-__device__ __forceinline__ float e4m3_value(uint8_t code) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
-}
-
-// One 16 x 16 tile of outputs per block, a thread per output; the sum of a group of 128 channels is scaled and added.
-template <bool kBf16>
-__global__ void __launch_bounds__(256)
-gemm_fp8_kernel(const ProductArgs g) {
-    __shared__ float a_tile[16][17], w_tile[16][17];
-    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint32_t row = blockIdx.y * 16 + ty, column = blockIdx.x * 16 + tx;
-    const uint32_t w_row = blockIdx.x * 16 + ty;
-    float total = 0.0f;
-    for (uint32_t group = 0; group < g.k_groups; group++) {
-        float part = 0.0f;
-        for (uint32_t k0 = group * kGroup; k0 < group * kGroup + kGroup; k0 += 16) {
-            const uint32_t k = k0 + tx;
-            a_tile[ty][tx] = row < g.m && k < g.k ? e4m3_value(g.a[row * g.a_stride + k]) : 0.0f;
-            w_tile[ty][tx] = w_row < g.n && k < g.k ? e4m3_value(g.w[w_row * g.w_stride + k]) : 0.0f;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 16; i++) part = fmaf(a_tile[ty][i], w_tile[tx][i], part);
-            __syncthreads();
-        }
-        if (row < g.m && column < g.n)
-            total += part * (g.a_scale[static_cast<size_t>(row) * g.k_groups + group] * g.w_scale[static_cast<size_t>(column / kGroup) * g.k_groups + group]);
-    }
-    if (row < g.m && column < g.n) g.c[row * g.c_stride + column] = bits_of<kBf16>(total);
-}
-
 }  // namespace
 }  // namespace krea2
 
@@ -244,33 +204,4 @@ extern "C" int krea2_prepare_plain_fp8(krea2_stream stream, size_t tokens, const
                            static_cast<uint32_t>(tokens), static_cast<uint32_t>(width), static_cast<uint32_t>((width + kGroup - 1) / kGroup),
                            x_stride, 0, 0, out_stride, 0.0f, 0.0f};
     return run_prepare<false>(name, static_cast<cudaStream_t>(stream), g, kind);
-}
-
-extern "C" int krea2_gemm_fp8_128(krea2_stream stream, size_t m, const void *a, const void *w, const float *scale, const float *a_scale,
-                                  void *c, size_t k_size, size_t a_stride, size_t w_stride, size_t n_size, size_t c_stride, int kind) {
-    clear_error();
-    const char *name = "gemm_fp8_128";
-    KREA2_REQUIRE(m >= 1 && m <= 16777216, "%s: m %zu outside 1..16777216", name, m);
-    KREA2_REQUIRE(k_size >= 1 && k_size <= 65536, "%s: k_size %zu outside 1..65536", name, k_size);
-    KREA2_REQUIRE(n_size >= 1 && n_size <= 262144, "%s: n_size %zu outside 1..262144", name, n_size);
-    KREA2_REQUIRE(a_stride >= k_size && a_stride % 16 == 0, "%s: a_stride %zu must be a multiple of 16, at least k_size %zu", name, a_stride, k_size);
-    KREA2_REQUIRE(w_stride >= k_size && w_stride % 16 == 0, "%s: w_stride %zu must be a multiple of 16, at least k_size %zu", name, w_stride, k_size);
-    KREA2_REQUIRE(c_stride >= n_size, "%s: c_stride %zu is below n_size %zu", name, c_stride, n_size);
-    KREA2_REQUIRE(kind == KREA2_F16 || kind == KREA2_BF16, "%s: kind %d is neither KREA2_F16 nor KREA2_BF16", name, kind);
-    KREA2_REQUIRE(a && w && scale && a_scale && c, "%s: null buffer", name);
-    KREA2_REQUIRE(aligned16(a) && aligned16(w), "%s: the codes must be 16-byte aligned", name);
-    KREA2_REQUIRE(reinterpret_cast<uintptr_t>(c) % 2 == 0 && reinterpret_cast<uintptr_t>(scale) % 4 == 0 &&
-                      reinterpret_cast<uintptr_t>(a_scale) % 4 == 0,
-                  "%s: buffers must be aligned to their element size", name);
-    const ProductArgs g = {static_cast<const uint8_t *>(a), static_cast<const uint8_t *>(w), scale, a_scale, static_cast<uint16_t *>(c),
-                           static_cast<uint32_t>(m), static_cast<uint32_t>(n_size), static_cast<uint32_t>(k_size),
-                           static_cast<uint32_t>((k_size + kGroup - 1) / kGroup), a_stride, w_stride, c_stride};
-    KREA2_REQUIRE((m + 15) / 16 <= 65535, "%s: m %zu is too large", name, m);
-    const dim3 grid(static_cast<unsigned>((n_size + 15) / 16), static_cast<unsigned>((m + 15) / 16));
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (kind == KREA2_BF16) gemm_fp8_kernel<true><<<grid, 256, 0, s>>>(g);
-    else gemm_fp8_kernel<false><<<grid, 256, 0, s>>>(g);
-    const cudaError_t status = cudaGetLastError();
-    if (status != cudaSuccess) return fail(KREA2_RUNTIME, "%s launch failed: %s", name, cudaGetErrorString(status));
-    return KREA2_OK;
 }
