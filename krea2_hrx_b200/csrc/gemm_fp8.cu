@@ -10,6 +10,8 @@
 //   narrow  few rows of a: 128 rows of w are the M side and up to 256 rows of a the N side of a CTA, the blocks of 128
 //           channels are split over a cluster of up to eight CTAs, whose partial outputs are added over distributed shared
 //           memory in the order of their rank: no workspace, no atomics, the same bits every time
+#include <atomic>
+
 #include "tensor_core.cuh"
 
 namespace krea2 {
@@ -52,27 +54,99 @@ __device__ __forceinline__ void issue_product(uint32_t tmem, uint64_t a, uint64_
                      : "memory");
 }
 
-// ---------------------------------------------------------------- wide
-struct Wide {
-    static constexpr int kStages = 6;
-    static constexpr int kRows = 128;     // of a, and of w, per CTA
-    static constexpr int kColumns = 256;  // of a tile
-    static constexpr int kWarps = 8;      // epilogue: two per 32-lane quarter, each with half of the columns
-    static constexpr int kThreads = (kWarps + 2) * 32;
-    static constexpr int kOperandBytes = kRows * kBlock;
-    static constexpr int kStageBytes = 2 * kOperandBytes;
-    static constexpr int kStagingRow = 80;             // 32 outputs, and 16 bytes that spread the rows over the banks
-    static constexpr int kStagingBytes = 32 * kStagingRow;  // per warp
-    static constexpr int kSharedBytes = kStages * kStageBytes + 1024 + 256 + kWarps * kStagingBytes;
+// ---------------------------------------------------------------- scales
+// The rows' scales lie [row][block]: a warp that loads one block's for 32 rows touches 32 lines, and eight epilogue warps
+// doing so take the L1's whole time.  So two warps of a CTA load four blocks at a time (16 bytes a row) and lay them out
+// [block][row] in a ring in shared memory for all.
+template <int kRows, bool kMultiply>
+struct ScaleRing {
+    static constexpr int kSlots = 3, kRun = 4;                // runs of four blocks
+    static constexpr int kWarps = 2, kPerLane = (kRows + 63) / 64;
+    static constexpr int kSlotFloats = kRun * kRows + 8;      // and each block's scale of w (of either half), if not multiplied in
+    static constexpr int kBytes = kSlots * kSlotFloats * 4;
+    float *values;
+    uint64_t *full, *empty;
+
+    __device__ __forceinline__ float *slot(uint32_t run) const { return values + (run % kSlots) * kSlotFloats; }
+    __device__ __forceinline__ static uint32_t parity(uint32_t run) { return (run / kSlots) & 1u; }
+
+    // Blocks first .. last - 1 of the rows from row0 on, by warp `which` of the two.  `w0`, `w1`: the scales of w (w1 of the
+    // second half, not multiplied in).  False when a wait ran out.
+    __device__ __forceinline__ bool fill(const float *a_scale, const float *w0, const float *w1, uint32_t row0, uint32_t m, uint32_t blocks, uint32_t first,
+                                         uint32_t last, int which, int lane, uint32_t &run, const Abort &abort) const {
+        const bool vector = ((blocks | first) & 3u) == 0u && (reinterpret_cast<uintptr_t>(a_scale) & 15u) == 0u;
+        const float *from[kPerLane];
+#pragma unroll
+        for (int i = 0; i < kPerLane; i++)
+            from[i] = a_scale + static_cast<size_t>(min(row0 + (2 * i + which) * 32 + lane, m - 1)) * blocks;
+        float4 ahead[kPerLane];
+        auto request = [&](uint32_t b) {
+#pragma unroll
+            for (int i = 0; i < kPerLane; i++) {
+                if (vector) {
+                    ahead[i] = __ldg(reinterpret_cast<const float4 *>(from[i] + b));
+                } else {
+                    ahead[i].x = __ldg(from[i] + b), ahead[i].y = __ldg(from[i] + min(b + 1, last - 1));
+                    ahead[i].z = __ldg(from[i] + min(b + 2, last - 1)), ahead[i].w = __ldg(from[i] + min(b + 3, last - 1));
+                }
+            }
+        };
+        request(first);
+        for (uint32_t b = first; b < last; b += kRun, run++) {
+            if (!barrier_wait_warp(empty + run % kSlots, parity(run) ^ 1u, abort)) return false;
+            float *to = slot(run);
+            float w[kRun];
+            if constexpr (kMultiply) {
+#pragma unroll
+                for (int k = 0; k < kRun; k++) w[k] = __ldg(w0 + min(b + k, last - 1));
+            } else if (which == 0 && lane < 8) {
+                to[kRun * kRows + lane] = __ldg((lane < 4 ? w0 : w1) + min(b + (lane & 3), last - 1));
+            }
+#pragma unroll
+            for (int i = 0; i < kPerLane; i++) {
+                const int row = (2 * i + which) * 32 + lane;
+                const float v[kRun] = {ahead[i].x, ahead[i].y, ahead[i].z, ahead[i].w};
+                if (row < kRows)
+#pragma unroll
+                    for (int k = 0; k < kRun; k++) to[k * kRows + row] = kMultiply ? v[k] * w[k] : v[k];
+            }
+            __syncwarp();
+            if (lane == 0) barrier_arrive(full + run % kSlots);
+            if (b + kRun < last) request(b + kRun);
+        }
+        return true;
+    }
 };
 
-// Writes 32 outputs of each of the warp's 32 rows through its staging area, so that rows leave in 64-byte pieces.
+// ---------------------------------------------------------------- wide
+struct Wide {
+    static constexpr int kRows = 128;     // of a, and of w, per CTA
+    static constexpr int kColumns = 256;  // of a tile
+    static constexpr int kStages = 6;
+    static constexpr int kWarps = 8;      // epilogue: two per 32-lane quarter, each with half of the columns
+    using Scales = ScaleRing<kRows, false>;
+    static constexpr int kWarpColumns = kColumns / (kWarps / 4);
+    static constexpr int kThreads = (kWarps + 4) * 32;  // a warpgroup beside them: one loads, one issues, two lay out scales
+    // The launch gives each thread 168 registers; the epilogue's two warpgroups, with 128 outputs a thread, take some of
+    // the third's.
+    static constexpr int kEpilogueRegisters = 208, kOtherRegisters = 64;
+    static_assert((kWarps / 4) * kEpilogueRegisters + kOtherRegisters <= (kWarps / 4 + 1) * 168, "registers of the launch");
+    static constexpr int kOperandBytes = kRows * kBlock;
+    static constexpr int kStageBytes = 2 * kOperandBytes;
+    static constexpr int kStagingBytes = 32 * 64;  // per warp: 32 rows of 32 outputs on their way out
+    static constexpr int kSharedBytes = kStages * kStageBytes + 1024 + 256 + kWarps * kStagingBytes + Scales::kBytes;
+    static_assert(kSharedBytes <= 227 * 1024, "shared memory");
+};
+
+// Writes 32 outputs of each of the warp's 32 rows through its staging area, so that rows leave in 64-byte pieces; the
+// 16-byte pieces of a row change places from one pair of rows to the next, which spreads a column of them over the banks.
 __device__ __forceinline__ void store_wide(const ProductArgs &g, const float2 *values, uint32_t row0, uint32_t column0, uint8_t *staging, int lane) {
-    uint4 *mine = reinterpret_cast<uint4 *>(staging + lane * Wide::kStagingRow);
+    auto piece = [&](uint32_t row, uint32_t i) { return staging + row * 64 + ((i ^ ((row >> 1) & 3u)) * 16); };
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        mine[i] = make_uint4(pack_outputs(values[4 * i].x, values[4 * i].y, g.bf16), pack_outputs(values[4 * i + 1].x, values[4 * i + 1].y, g.bf16),
-                             pack_outputs(values[4 * i + 2].x, values[4 * i + 2].y, g.bf16), pack_outputs(values[4 * i + 3].x, values[4 * i + 3].y, g.bf16));
+    for (uint32_t i = 0; i < 4; i++)
+        *reinterpret_cast<uint4 *>(piece(lane, i)) =
+            make_uint4(pack_outputs(values[4 * i].x, values[4 * i].y, g.bf16), pack_outputs(values[4 * i + 1].x, values[4 * i + 1].y, g.bf16),
+                       pack_outputs(values[4 * i + 2].x, values[4 * i + 2].y, g.bf16), pack_outputs(values[4 * i + 3].x, values[4 * i + 3].y, g.bf16));
     __syncwarp();
     if (g.aligned) {
         const uint32_t column = column0 + (lane & 3) * 8;
@@ -80,7 +154,7 @@ __device__ __forceinline__ void store_wide(const ProductArgs &g, const float2 *v
         for (int r = 0; r < 32; r += 8) {
             const uint32_t local = r + (lane >> 2), row = row0 + local;
             if (row >= g.m || column >= g.n) continue;
-            const uint8_t *from = staging + local * Wide::kStagingRow + (lane & 3) * 16;
+            const uint8_t *from = piece(local, lane & 3);
             uint16_t *to = g.c + row * g.c_stride + column;
             if (column + 8 <= g.n) {
                 *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
@@ -90,7 +164,7 @@ __device__ __forceinline__ void store_wide(const ProductArgs &g, const float2 *v
         }
     } else if (column0 + lane < g.n) {
         for (uint32_t local = 0; local < 32 && row0 + local < g.m; local++)
-            g.c[(row0 + local) * g.c_stride + column0 + lane] = reinterpret_cast<const uint16_t *>(staging + local * Wide::kStagingRow)[lane];
+            g.c[(row0 + local) * g.c_stride + column0 + lane] = reinterpret_cast<const uint16_t *>(piece(local, lane >> 3))[lane & 7];
     }
     __syncwarp();
 }
@@ -101,12 +175,14 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     extern __shared__ uint8_t shared_raw[];
     uint8_t *shared = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(shared + T::kStages * T::kStageBytes);
-    uint64_t *empty = full + T::kStages, *sum_full = empty + T::kStages, *sum_empty = sum_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sum_empty + 2);
+    uint64_t *empty = full + T::kStages, *sum_full = empty + T::kStages, *sum_empty = sum_full + 4;  // [half][parity]
+    uint64_t *scale_full = sum_empty + 4, *scale_empty = scale_full + T::Scales::kSlots;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_empty + T::Scales::kSlots);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     // [0], [1] the stages each CTA's producer filled (in the leader), [2], [3] each CTA's abort flag (in both)
     volatile uint32_t *exchange = reinterpret_cast<volatile uint32_t *>(tmem_slot + 2);
     uint8_t *staging = shared + T::kStages * T::kStageBytes + 256;
+    const T::Scales scales = {reinterpret_cast<float *>(staging + T::kWarps * T::kStagingBytes), scale_full, scale_empty};
     const Abort abort = {abort_flag, &g_product_status, kProductTimedOut};
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -133,9 +209,13 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             barrier_init(full + s, 1);
             barrier_init(empty + s, 1);
         }
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < 4; s++) {
             barrier_init(sum_full + s, 1);
-            barrier_init(sum_empty + s, 2 * T::kWarps);
+            barrier_init(sum_empty + s, T::kWarps);  // the half's warps of both CTAs
+        }
+        for (int s = 0; s < T::Scales::kSlots; s++) {
+            barrier_init(scale_full + s, T::Scales::kWarps);
+            barrier_init(scale_empty + s, T::kWarps);
         }
         *abort_flag = 0;
         barrier_init_done();
@@ -148,9 +228,9 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     cluster_barrier();
     tensor_fence_after();
     const uint32_t tmem = *tmem_slot;
-
-    if (warp == T::kWarps) {
-        if (lane == 0) {
+    if (warp >= T::kWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegisters));
+        if (warp == T::kWarps && lane == 0) {
             uint32_t stage = 0, phase = 0;
             bool alive = true;
             for (uint32_t tile = pair; alive && tile < tiles; tile += pairs) {
@@ -162,73 +242,103 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     const uint32_t leader_full = cluster_address(full + stage, 0);
                     if (leader) barrier_expect(full + stage, 2 * T::kStageBytes);
                     load_tile_pair(dst, &map_a, leader_full, static_cast<int>(b * kBlock), static_cast<int>(row));
-                    load_tile_pair(dst + T::kOperandBytes, &map_w, leader_full, static_cast<int>(b * kBlock), static_cast<int>(column + rank * T::kRows));
+                    // this CTA's 64 rows of either half
+                    load_tile_pair(dst + T::kOperandBytes, &map_w, leader_full, static_cast<int>(b * kBlock), static_cast<int>(column + rank * 64));
+                    load_tile_pair(dst + T::kOperandBytes + T::kOperandBytes / 2, &map_w, leader_full, static_cast<int>(b * kBlock),
+                                   static_cast<int>(column + kBlock + rank * 64));
                     issued++;
                     if (++stage == T::kStages) stage = 0, phase ^= 1u;
                 }
             }
         }
-    } else if (warp == T::kWarps + 1) {
-        if (leader && lane == 0) {
-            constexpr uint32_t idesc = product_descriptor(2 * T::kRows, T::kColumns);
+        if (warp == T::kWarps + 1 && leader) {
+            const bool elected = elect_lane();
+            constexpr uint32_t idesc = product_descriptor(2 * T::kRows, T::kColumns / 2);
             uint32_t stage = 0, phase = 0, count = 0;
             bool alive = true;
             for (uint32_t tile = pair; alive && tile < tiles; tile += pairs) {
                 for (uint32_t b = 0; b < g.blocks; b++, count++) {
                     const uint32_t s = count & 1u;
-                    if (!(alive = barrier_wait(sum_empty + s, ((count >> 1) & 1u) ^ 1u, abort) && barrier_wait(full + stage, phase, abort))) break;
-                    tensor_fence_after();
                     const uint32_t at = smem_address(shared + stage * T::kStageBytes);
-                    const uint64_t a = operand_descriptor(at), w = operand_descriptor(at + T::kOperandBytes);
+                    const uint64_t a = operand_descriptor(at);
 #pragma unroll
-                    for (int k = 0; k < kBlock / kStep; k++) issue_product<2>(tmem + s * T::kColumns, a + 2 * k, w + 2 * k, idesc, k != 0);
-                    tensor_commit_pair(empty + stage);
-                    tensor_commit_pair(sum_full + s);
+                    for (uint32_t half = 0; half < 2; half++) {
+                        if (!(alive = alive && barrier_wait_warp(sum_empty + 2 * half + s, ((count >> 1) & 1u) ^ 1u, abort) &&
+                                      (half != 0 || barrier_wait_warp(full + stage, phase, abort))))
+                            break;
+                        tensor_fence_after();
+                        // each CTA holds 128 of the tile's rows of w: its 64 of this half lie at 64 * half
+                        const uint64_t w = operand_descriptor(at + T::kOperandBytes + half * (T::kOperandBytes / 2));
+                        if (elected) {
+#pragma unroll
+                            for (int k = 0; k < kBlock / kStep; k++)
+                                issue_product<2>(tmem + s * T::kColumns + half * kBlock, a + 2 * k, w + 2 * k, idesc, k != 0);
+                            tensor_commit_pair(sum_full + 2 * half + s);
+                            if (half == 1) tensor_commit_pair(empty + stage);
+                        }
+                        __syncwarp();
+                    }
+                    if (!alive) break;
                     if (++stage == T::kStages) stage = 0, phase ^= 1u;
                 }
             }
         }
+        if (warp >= T::kWarps + 2) {
+            uint32_t run = 0;
+            const uint32_t scale_rows = (g.n + kBlock - 1) / kBlock;
+            for (uint32_t tile = pair; tile < tiles; tile += pairs) {
+                uint32_t row, column;
+                origin(tile, row, column);
+                const float *w0 = g.w_scale + static_cast<size_t>(column / kBlock) * g.blocks;
+                const float *w1 = column / kBlock + 1 < scale_rows ? w0 + g.blocks : w0;
+                if (!scales.fill(g.a_scale, w0, w1, row, g.m, g.blocks, 0, g.blocks, warp - T::kWarps - 2, lane, run, abort)) break;
+            }
+        }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kEpilogueRegisters));
         const int quarter = warp & 3, half = warp >> 2;
-        uint32_t count = 0;
+        uint32_t count = 0, run = 0;
         bool alive = true;
-        const uint32_t scale_rows = (g.n + kBlock - 1) / kBlock;
+        const uint32_t release[2] = {cluster_address(sum_empty + 2 * half, 0), cluster_address(sum_empty + 2 * half + 1, 0)};
         for (uint32_t tile = pair; alive && tile < tiles; tile += pairs) {
             uint32_t row0, column0;
             origin(tile, row0, column0);
             row0 += quarter * 32;
-            column0 += half * kBlock;
-            const uint32_t row = min(row0 + lane, g.m - 1), scale_row = min(column0 / kBlock, scale_rows - 1);
-            const float *a_scale = g.a_scale + static_cast<size_t>(row) * g.blocks, *w_scale = g.w_scale + static_cast<size_t>(scale_row) * g.blocks;
-            float2 out[64];
+            column0 += half * T::kWarpColumns;
+            float2 out[T::kWarpColumns / 2];
 #pragma unroll
-            for (int i = 0; i < 64; i++) out[i] = make_float2(0.0f, 0.0f);
-            float next = __ldg(a_scale) * __ldg(w_scale);
+            for (int i = 0; i < T::kWarpColumns / 2; i++) out[i] = make_float2(0.0f, 0.0f);
             for (uint32_t b = 0; b < g.blocks; b++, count++) {
                 const uint32_t s = count & 1u;
-                const float2 scale = make_float2(next, next);
-                if (b + 1 < g.blocks) next = __ldg(a_scale + b + 1) * __ldg(w_scale + b + 1);
-                alive = __all_sync(0xffffffffu, barrier_wait(sum_full + s, (count >> 1) & 1u, abort));
-                if (!alive) break;
+                if ((b & 3u) == 0u && !(alive = barrier_wait_warp(scale_full + run % T::Scales::kSlots, T::Scales::parity(run), abort))) break;
+                const float *run_scales = scales.slot(run);
+                const float one = run_scales[(b & 3u) * T::kRows + quarter * 32 + lane] * run_scales[4 * T::kRows + half * 4 + (b & 3u)];
+                const float2 scale = make_float2(one, one);
+                if ((b & 3u) == 3u || b + 1 == g.blocks) {
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(scale_empty + run % T::Scales::kSlots);
+                    run++;
+                }
+                if (!(alive = barrier_wait_warp(sum_full + 2 * half + s, (count >> 1) & 1u, abort))) break;
                 tensor_fence_after();
-                const uint32_t from = tmem + s * T::kColumns + half * kBlock + (static_cast<uint32_t>(quarter * 32) << 16);
+                const uint32_t from = tmem + s * T::kColumns + half * T::kWarpColumns + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    float part[16];
-                    tensor_load_16(from + c * 16, part);
+                for (int c = 0; c < T::kWarpColumns / 16; c++) {
+                    float sums[16];
+                    tensor_load_16(from + c * 16, sums);
                     tensor_loads_done();
-                    if (c == 7) {  // everything has been read: the accumulator may be overwritten
+                    if (c == T::kWarpColumns / 16 - 1) {  // everything has been read: the accumulator may be overwritten
                         tensor_fence_before();
                         __syncwarp();
-                        if (lane == 0) barrier_arrive_at(cluster_address(sum_empty + s, 0));
+                        if (lane == 0) barrier_arrive_at(release[s]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) out[c * 8 + i] = fma_pair(make_float2(part[2 * i], part[2 * i + 1]), scale, out[c * 8 + i]);
+                    for (int i = 0; i < 8; i++) out[c * 8 + i] = fma_pair(make_float2(sums[2 * i], sums[2 * i + 1]), scale, out[c * 8 + i]);
                 }
             }
             if (!alive) break;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+            for (int c = 0; c < T::kWarpColumns / 32; c++)
                 store_wide(g, out + c * 16, row0, column0 + c * 32, staging + warp * T::kStagingBytes, lane);
         }
     }
@@ -273,17 +383,23 @@ constexpr int power_of_two(int n) { return n <= 32 ? 32 : 2 * power_of_two((n + 
 template <int kTokens>
 struct Narrow {
     static constexpr int kRows = 128;                        // of w
-    static constexpr int kWarps = kTokens <= 64 ? 4 : 8;     // epilogue
-    static constexpr int kThreads = (kWarps + 2) * 32;
+    static constexpr int kWarps = kTokens <= 32 ? 4 : kTokens <= 192 ? 8 : 16;  // epilogue
+    static constexpr int kThreads = (kWarps + 4) * 32;       // and one warp that loads, one that issues, two that lay out scales
+    using Scales = ScaleRing<kTokens, true>;
     static constexpr int kColumns = kTokens / (kWarps / 4);  // tokens of one epilogue thread
     static constexpr int kStageBytes = (kRows + kTokens) * kBlock;
-    // Two CTAs share an SM where both sets of accumulators fit its tensor memory (512 columns, 2 * kTokens each): their
-    // shared memory has to keep a second one out otherwise, since a CTA that waits for tensor memory holds up its cluster.
-    static constexpr int kTensorColumns = power_of_two(2 * kTokens);
-    static constexpr int kPerSm = kTensorColumns <= 256 ? 2 : 1;
-    static constexpr int kStages = ((kPerSm == 2 ? 108 : 216) * 1024 - 2048 - 2 * kTokens * 4) / kStageBytes;
-    static constexpr int kSharedBytes = kStages * kStageBytes + 1024 + 256 + 2 * kTokens * 4;
-    static_assert(kStages >= 2 && kStages * kStageBytes >= kRows * kTokens * 4, "the partial outputs take the stages' place");
+    // Up to 64 tokens two CTAs share an SM, so that one streams while the other starts or adds up.  Above, a thread's
+    // outputs want the registers of one; and where two sets of accumulators exceed tensor memory (512 columns, 2 * kTokens
+    // each) the shared memory has to keep the second out, since a CTA that waits for tensor memory holds up its cluster.
+    static constexpr int kPerSm = kTokens <= 64 ? 2 : 1;
+    // Blocks between the products and the epilogue: each is short, and the way to the epilogue's warps and back long.
+    static constexpr int kSums = kTokens <= 32 ? 8 : kTokens <= 128 ? 4 : kTokens <= 160 ? 3 : 2;
+    static constexpr int kTensorColumns = power_of_two(kSums * kTokens);
+    static_assert(kPerSm * kTensorColumns <= 512, "tensor memory");
+    static constexpr int kStages = ((kPerSm == 2 ? 108 : 216) * 1024 - 2048 - Scales::kBytes) / kStageBytes;
+    static constexpr int kSharedBytes = kStages * kStageBytes + 1024 + 512 + Scales::kBytes;
+    static constexpr int kPitch = kRows + 4;  // of the partial outputs, in floats: a fragment's four tokens fall into different banks
+    static_assert(kStages >= 2 && kStages * kStageBytes >= kPitch * kTokens * 4, "the partial outputs take the stages' place");
     static_assert(kPerSm * kSharedBytes <= 227 * 1024 && (kPerSm + 1) * (kSharedBytes + 1024) > 228 * 1024, "CTAs per SM");
 };
 
@@ -294,11 +410,12 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     extern __shared__ uint8_t shared_raw[];
     uint8_t *shared = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(shared + T::kStages * T::kStageBytes);
-    uint64_t *empty = full + T::kStages, *sum_full = empty + T::kStages, *sum_empty = sum_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sum_empty + 2);
+    uint64_t *empty = full + T::kStages, *sum_full = empty + T::kStages, *sum_empty = sum_full + T::kSums;
+    uint64_t *scale_full = sum_empty + T::kSums, *scale_empty = scale_full + T::Scales::kSlots;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(scale_empty + T::Scales::kSlots);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    float *scales = reinterpret_cast<float *>(shared + T::kStages * T::kStageBytes + 256);  // two blocks' token scales
-    float *partial = reinterpret_cast<float *>(shared);                                     // [kTokens][128], once the stages are done with
+    const typename T::Scales scales = {reinterpret_cast<float *>(shared + T::kStages * T::kStageBytes + 512), scale_full, scale_empty};
+    float *partial = reinterpret_cast<float *>(shared);                                     // [kTokens][kPitch], once the stages are done with
     const Abort abort = {abort_flag, &g_product_status, kProductTimedOut};
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -313,9 +430,13 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             barrier_init(full + s, 1);
             barrier_init(empty + s, 1);
         }
-        for (int s = 0; s < 2; s++) {
+        for (int s = 0; s < T::kSums; s++) {
             barrier_init(sum_full + s, 1);
             barrier_init(sum_empty + s, T::kWarps);
+        }
+        for (int s = 0; s < T::Scales::kSlots; s++) {
+            barrier_init(scale_full + s, T::Scales::kWarps);
+            barrier_init(scale_empty + s, T::kWarps);
         }
         *abort_flag = 0;
         barrier_init_done();
@@ -341,47 +462,55 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             }
         }
     } else if (warp == T::kWarps + 1) {
-        if (lane == 0) {
+        {
+            const bool elected = elect_lane();
             constexpr uint32_t idesc = product_descriptor(T::kRows, kTokens);
             for (uint32_t b = first, count = 0; b < last; b++, count++) {
-                const uint32_t s = count & 1u, stage = count % T::kStages;
-                if (!barrier_wait(sum_empty + s, ((count >> 1) & 1u) ^ 1u, abort) || !barrier_wait(full + stage, (count / T::kStages) & 1u, abort)) break;
+                const uint32_t s = count % T::kSums, stage = count % T::kStages;
+                if (!barrier_wait_warp(sum_empty + s, ((count / T::kSums) & 1u) ^ 1u, abort) || !barrier_wait_warp(full + stage, (count / T::kStages) & 1u, abort)) break;
                 tensor_fence_after();
                 const uint32_t at = smem_address(shared + stage * T::kStageBytes);
                 const uint64_t w = operand_descriptor(at), a = operand_descriptor(at + T::kRows * kBlock);
+                if (elected) {
 #pragma unroll
-                for (int k = 0; k < kBlock / kStep; k++) issue_product<1>(tmem + s * kTokens, w + 2 * k, a + 2 * k, idesc, k != 0);
-                tensor_commit(empty + stage);
-                tensor_commit(sum_full + s);
+                    for (int k = 0; k < kBlock / kStep; k++) issue_product<1>(tmem + s * kTokens, w + 2 * k, a + 2 * k, idesc, k != 0);
+                    tensor_commit(empty + stage);
+                    tensor_commit(sum_full + s);
+                }
+                __syncwarp();
             }
         }
-    } else {
-        // A thread owns one row of w and kColumns tokens.  The tokens' scales of a block (times the weights', which the
-        // whole CTA shares) lie in shared memory, two blocks of them in turn.
-        const int quarter = warp & 3, group = warp >> 2;
+    } else if (warp >= T::kWarps + 2) {
+        uint32_t run = 0;
         const float *w_scale = g.w_scale + static_cast<size_t>(blockIdx.y) * g.blocks;
-        const uint32_t token = threadIdx.x;
-        const float *a_scale = g.a_scale + static_cast<size_t>(min(m0 + token, g.m - 1)) * g.blocks;
-        const bool loads = token < kTokens;
-        float2 out[T::kColumns / 2];
+        scales.fill(g.a_scale, w_scale, w_scale, m0, g.m, g.blocks, first, last, warp - T::kWarps - 2, lane, run, abort);
+    } else {
+        // A warp owns 32 rows of w and kColumns tokens, a thread four of the rows (lane / 4 + 0, 8, 16, 24) and every
+        // fourth pair of tokens, so that a scale it reads from shared memory serves four outputs.  (With a row and all
+        // tokens per thread, each scale is handed to 32 lanes for one output each: four clocks of shared memory a token
+        // and block, twice what the product takes.)
+        const int quarter = warp & 3, group = warp >> 2;
+        float2 out[T::kColumns / 8][4];
 #pragma unroll
-        for (int i = 0; i < T::kColumns / 2; i++) out[i] = make_float2(0.0f, 0.0f);
-        float next = loads ? __ldg(a_scale + first) * __ldg(w_scale + first) : 0.0f;
+        for (int i = 0; i < T::kColumns / 8; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) out[i][r] = make_float2(0.0f, 0.0f);
+        uint32_t run = 0;
         for (uint32_t b = first, count = 0; b < last; b++, count++) {
-            const uint32_t s = count & 1u;
-            if (loads) {
-                scales[s * kTokens + token] = next;
-                if (b + 1 < last) next = __ldg(a_scale + b + 1) * __ldg(w_scale + b + 1);
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(T::kWarps * 32) : "memory");
-            if (!__all_sync(0xffffffffu, barrier_wait(sum_full + s, (count >> 1) & 1u, abort))) *abort_flag = 1;  // all leave the loop below
+            const uint32_t s = count % T::kSums, k = count & 3u;
+            if (k == 0u && !barrier_wait_warp(scale_full + run % T::Scales::kSlots, T::Scales::parity(run), abort)) break;
+            if (!barrier_wait_warp(sum_full + s, (count / T::kSums) & 1u, abort)) break;
             tensor_fence_after();
             const uint32_t from = tmem + s * kTokens + group * T::kColumns + (static_cast<uint32_t>(quarter * 32) << 16);
-            const float *mine = scales + s * kTokens + group * T::kColumns;
+            const float *mine = scales.slot(run) + k * kTokens + group * T::kColumns + 2 * (lane & 3);
 #pragma unroll
             for (int c = 0; c < T::kColumns; c += 16) {
-                float part[16];
-                tensor_load_16(from + c, part);
+                float sums[2][8];
+                tensor_load_fragment(from + c, sums[0]);
+                tensor_load_fragment(from + c + (16u << 16), sums[1]);
+                float2 scale[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) scale[j] = *reinterpret_cast<const float2 *>(mine + c + 8 * j);
                 tensor_loads_done();
                 if (c + 16 == T::kColumns) {
                     tensor_fence_before();
@@ -389,23 +518,30 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     if (lane == 0) barrier_arrive(sum_empty + s);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 scale = *reinterpret_cast<const float4 *>(mine + c + 4 * i);
-                    float2 &lo = out[(c + 4 * i) / 2], &hi = out[(c + 4 * i) / 2 + 1];
-                    lo = fma_pair(make_float2(part[4 * i], part[4 * i + 1]), make_float2(scale.x, scale.y), lo);
-                    hi = fma_pair(make_float2(part[4 * i + 2], part[4 * i + 3]), make_float2(scale.z, scale.w), hi);
-                }
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float *sum = sums[r >> 1] + 4 * j + 2 * (r & 1);
+                        out[c / 8 + j][r] = fma_pair(make_float2(sum[0], sum[1]), scale[j], out[c / 8 + j][r]);
+                    }
+            }
+            if (k == 3u || b + 1 == last) {
+                __syncwarp();
+                if (lane == 0) barrier_arrive(scale_empty + run % T::Scales::kSlots);
+                run++;
             }
         }
         // The last sum has been read, so every product has read its stage and every load has landed.
         asm volatile("bar.sync 1, %0;" ::"n"(T::kWarps * 32) : "memory");
         if (!*abort_flag) {
-            const uint32_t row = quarter * 32 + lane;
+            float *to = partial + (group * T::kColumns + 2 * (lane & 3)) * T::kPitch + quarter * 32 + lane / 4;
 #pragma unroll
-            for (int i = 0; i < T::kColumns / 2; i++) {
-                partial[(group * T::kColumns + 2 * i) * T::kRows + row] = out[i].x;
-                partial[(group * T::kColumns + 2 * i + 1) * T::kRows + row] = out[i].y;
-            }
+            for (int i = 0; i < T::kColumns / 8; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    to[8 * i * T::kPitch + 8 * r] = out[i][r].x;
+                    to[(8 * i + 1) * T::kPitch + 8 * r] = out[i][r].y;
+                }
         }
     }
 
@@ -428,10 +564,13 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const uint32_t token = item / 32, column = n0 + (item % 32) * 4;
         if (m0 + token >= g.m || column >= g.n) continue;
         float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t r = 0; r < shares; r++) {
-            const float4 share = cluster_load(cluster_address(partial + item * 4, r));
-            total.x += share.x, total.y += share.y, total.z += share.z, total.w += share.w;
-        }
+        float4 share[8];  // requested together: a load from another CTA takes as long as one from L2
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++)
+            if (r < shares) share[r] = cluster_load(cluster_address(partial + token * T::kPitch + (item % 32) * 4, r));
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++)
+            if (r < shares) total.x += share[r].x, total.y += share[r].y, total.z += share[r].z, total.w += share[r].w;
         const uint2 packed = make_uint2(pack_outputs(total.x, total.y, g.bf16), pack_outputs(total.z, total.w, g.bf16));
         uint16_t *to = g.c + (m0 + token) * g.c_stride + column;
         if (g.aligned && column + 4 <= g.n) {
@@ -454,24 +593,70 @@ int operand_map(CUtensorMap *map, const void *base, size_t rows, size_t k, size_
 }
 
 template <int kTokens>
-int launch_narrow(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, uint32_t shares, const ProductArgs &g) {
+cudaLaunchConfig_t narrow_config(const ProductArgs &g, uint32_t shares, cudaLaunchAttribute &attribute) {
     using T = Narrow<kTokens>;
-    static Prepared prepared;
-    if (int status = prepare_kernel(prepared, narrow_kernel<kTokens>, T::kSharedBytes)) return status;
-    CUtensorMap map_a, map_w;
-    if (int status = operand_map(&map_a, a, g.m, k, a_stride, kTokens)) return status;
-    if (int status = operand_map(&map_w, w, g.n, k, w_stride, T::kRows)) return status;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(shares, (g.n + T::kRows - 1) / T::kRows, (g.m + kTokens - 1) / kTokens);
     config.blockDim = dim3(T::kThreads);
     config.dynamicSmemBytes = T::kSharedBytes;
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = shares;
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
+    return config;
+}
+
+// A launch of the narrow kernel and what it is expected to take.
+struct NarrowPlan {
+    uint32_t shares = 1;
+    float microseconds = 0.0f;
+};
+
+// The split of the blocks that keeps all clusters resident (more CTAs than that run in a second round, which costs more
+// than the shorter first one saves: 1 x 6144 x 6144 takes 10.6 us in four shares, 15.8 in six), and its time from
+// measured parts: a CTA's start and end 5 us, a block 0.18 us + 1.65 ns a token (a third more where two CTAs share an SM
+// that is full), and no less than its tiles take out of L2 at 13 TB/s.
+template <int kTokens>
+int plan_narrow(const ProductArgs &g, NarrowPlan *plan) {
+    using T = Narrow<kTokens>;
+    static Prepared prepared;
+    static std::atomic<int> known[64][9];  // clusters of so many CTAs that a device holds at once
+    if (int status = prepare_kernel(prepared, narrow_kernel<kTokens>, T::kSharedBytes)) return status;
+    int device = 0;
+    KREA2_CUDA(cudaGetDevice(&device));
+    const uint32_t tiles = ((g.n + T::kRows - 1) / T::kRows) * ((g.m + kTokens - 1) / kTokens);
+    uint32_t resident = 1;
+    for (uint32_t shares = 1; shares <= 8 && shares <= g.blocks; shares++) {
+        int clusters = known[device][shares].load(std::memory_order_relaxed);
+        if (clusters == 0) {
+            cudaLaunchAttribute attribute = {};
+            const cudaLaunchConfig_t config = narrow_config<kTokens>(g, shares, attribute);
+            KREA2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, narrow_kernel<kTokens>, &config));
+            if (clusters < 1) clusters = 1;
+            known[device][shares].store(clusters, std::memory_order_relaxed);
+        }
+        if (shares > 1 && tiles > static_cast<uint32_t>(clusters)) break;
+        plan->shares = shares;
+        resident = static_cast<uint32_t>(clusters);
+    }
+    const uint32_t rounds = (tiles + resident - 1) / resident, steps = (g.blocks + plan->shares - 1) / plan->shares;
+    const bool full = T::kPerSm == 2 && tiles * plan->shares > static_cast<uint32_t>(multiprocessors());
+    const float block = (0.18f + 0.00165f * kTokens) * (full ? 1.33f : 1.0f);
+    const float bytes = static_cast<float>(tiles) * g.blocks * T::kStageBytes;
+    const float busy = rounds * (steps * block + 5.0f) + 4.0f, fed = bytes / 13e6f + 9.0f;
+    plan->microseconds = busy > fed ? busy : fed;
+    return KREA2_OK;
+}
+
+template <int kTokens>
+int launch_narrow(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, uint32_t shares, const ProductArgs &g) {
+    CUtensorMap map_a, map_w;
+    if (int status = operand_map(&map_a, a, g.m, k, a_stride, kTokens)) return status;
+    if (int status = operand_map(&map_w, w, g.n, k, w_stride, Narrow<kTokens>::kRows)) return status;
+    cudaLaunchAttribute attribute = {};
+    cudaLaunchConfig_t config = narrow_config<kTokens>(g, shares, attribute);
+    config.stream = stream;
     const cudaError_t status = cudaLaunchKernelEx(&config, narrow_kernel<kTokens>, map_a, map_w, g);
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "gemm_fp8_128 launch failed: %s", cudaGetErrorString(status));
     return KREA2_OK;
@@ -483,7 +668,7 @@ int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, siz
     if (int status = prepare_kernel(prepared, wide_kernel, T::kSharedBytes)) return status;
     CUtensorMap map_a, map_w;
     if (int status = operand_map(&map_a, a, g.m, k, a_stride, T::kRows)) return status;
-    if (int status = operand_map(&map_w, w, g.n, k, w_stride, T::kRows)) return status;
+    if (int status = operand_map(&map_w, w, g.n, k, w_stride, T::kRows / 2)) return status;
     // As in the int8 product: while a stays in L2 a column of tiles is walked top to bottom, once it is larger than that
     // groups of w panels of up to 48 MB are walked row by row.
     if (static_cast<size_t>(g.m) * k > (size_t(48) << 20)) {
@@ -497,6 +682,50 @@ int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, siz
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "gemm_fp8_128 launch failed: %s", cudaGetErrorString(status));
     return KREA2_OK;
+}
+
+// The kernel and tile that are expected to take least.  The wide kernel takes 8 us and, for each round of tiles over the
+// pairs of SMs, 0.44 us a block.  It has the rows that fill its tiles: of 6144 columns and channels it takes 29 us for 128 to
+// 512 rows and 31 for 768, the narrow one (its best tile) 14 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512 and 47
+// for 768.  Beyond 1024 rows no shape's estimate chooses the narrow one.
+int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, const ProductArgs &g) {
+    NarrowPlan plan;
+#define KREA2_NARROW(tokens)                                                                       \
+    do {                                                                                           \
+        if (int status = plan_narrow<tokens>(g, &plan)) return status;                             \
+        return launch_narrow<tokens>(stream, a, w, k, a_stride, w_stride, plan.shares, g);         \
+    } while (0)
+    if (g.m <= 16) KREA2_NARROW(16);
+    if (g.m <= 32) KREA2_NARROW(32);
+#undef KREA2_NARROW
+    if (g.m <= 1024) {
+        const uint32_t tiles = ((g.m + 2 * Wide::kRows - 1) / (2 * Wide::kRows)) * ((g.n + Wide::kColumns - 1) / Wide::kColumns);
+        const uint32_t pairs = static_cast<uint32_t>(multiprocessors()) / 2;
+        float least = ((tiles + pairs - 1) / pairs) * (0.44f * g.blocks + 1.0f) + 8.0f;
+        int tokens = 0;
+        uint32_t shares = 1;
+#define KREA2_NARROW(candidate)                                                                    \
+    do {                                                                                           \
+        plan = NarrowPlan();                                                                       \
+        if (int status = plan_narrow<candidate>(g, &plan)) return status;                          \
+        if (plan.microseconds < least) least = plan.microseconds, tokens = candidate, shares = plan.shares; \
+    } while (0)
+        KREA2_NARROW(64);
+        if (g.m > 64) KREA2_NARROW(96);
+        if (g.m > 96) KREA2_NARROW(128);
+        if (g.m > 128) KREA2_NARROW(160);
+        if (g.m > 160) KREA2_NARROW(192);
+#undef KREA2_NARROW
+        switch (tokens) {
+            case 64: return launch_narrow<64>(stream, a, w, k, a_stride, w_stride, shares, g);
+            case 96: return launch_narrow<96>(stream, a, w, k, a_stride, w_stride, shares, g);
+            case 128: return launch_narrow<128>(stream, a, w, k, a_stride, w_stride, shares, g);
+            case 160: return launch_narrow<160>(stream, a, w, k, a_stride, w_stride, shares, g);
+            case 192: return launch_narrow<192>(stream, a, w, k, a_stride, w_stride, shares, g);
+            default: break;
+        }
+    }
+    return launch_wide(stream, a, w, k, a_stride, w_stride, g);
 }
 
 }  // namespace
@@ -534,14 +763,5 @@ extern "C" int krea2_gemm_fp8_128(krea2_stream stream, size_t m, const void *a, 
                            static_cast<uint32_t>((k_size + kBlock - 1) / kBlock), c_stride, kind == KREA2_BF16 ? 1u : 0u,
                            aligned16(c) && c_stride % 8 == 0 ? 1u : 0u, 0u};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (m > 256) return launch_wide(s, a, w, k_size, a_stride, w_stride, g);
-    // Narrow: as many shares as give each SM two CTAs of work, a block of channels each at least.
-    const uint32_t columns = (g.n + 127) / 128;
-    uint32_t shares = 1;
-    while (shares < 8 && 2 * shares <= g.blocks && columns * shares < 2u * static_cast<uint32_t>(multiprocessors())) shares *= 2;
-    if (m <= 16) return launch_narrow<16>(s, a, w, k_size, a_stride, w_stride, shares, g);
-    if (m <= 32) return launch_narrow<32>(s, a, w, k_size, a_stride, w_stride, shares, g);
-    if (m <= 64) return launch_narrow<64>(s, a, w, k_size, a_stride, w_stride, shares, g);
-    if (m <= 96) return launch_narrow<96>(s, a, w, k_size, a_stride, w_stride, shares, g);
-    return launch_narrow<128>(s, a, w, k_size, a_stride, w_stride, shares, g);
+    return launch_product(s, a, w, k_size, a_stride, w_stride, g);
 }

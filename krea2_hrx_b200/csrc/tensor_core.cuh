@@ -52,27 +52,54 @@ struct Abort {
     int *status;
     int bit;
 };
+// What a wait that has not been met does between its tests: every 64th time it looks whether the CTA gives up or the time
+// is over.  (The global timer takes longer to read than most waits last.)
+struct Patience {
+    uint64_t start = 0;
+    uint32_t spins = 0;
+    __device__ __forceinline__ bool over(const Abort &abort) {
+        if ((++spins & 63u) != 0u) return false;
+        if (*abort.flag) return true;
+        const uint64_t now = clock_ns();
+        if (start == 0) start = now;
+        if (now - start <= kTensorWaitLimitNs) return false;
+        *abort.flag = 1;
+        atomicOr(abort.status, abort.bit);
+        return true;
+    }
+};
 // Waits for the phase of `parity`.  False when the CTA is giving up, or when this wait ran out (it raises both flags).
 __device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity, const Abort &abort) {
-    if (barrier_test(bar, parity)) return true;
-    const uint64_t start = clock_ns();
-    for (uint32_t spin = 1;; ++spin) {
-        if (barrier_test(bar, parity)) return true;
-        if ((spin & 63u) == 0u) {
-            if (*abort.flag) return false;
-            if (clock_ns() - start > kTensorWaitLimitNs) {
-                *abort.flag = 1;
-                atomicOr(abort.status, abort.bit);
-                return false;
-            }
-        }
-    }
+    Patience patience;
+    while (!barrier_test(bar, parity))
+        if (patience.over(abort)) return false;
+    return true;
+}
+// The same for a converged warp, whose lanes leave together: 60 clocks where the phase is complete, 130 lane by lane.
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t *bar, uint32_t parity, const Abort &abort) {
+    Patience patience;
+    while (!__all_sync(0xffffffffu, barrier_test(bar, parity)))
+        if (__any_sync(0xffffffffu, patience.over(abort))) return false;
+    return true;
 }
 // After a wait that gave up: waits (bounded) until the loads armed on this phase have landed, so that none still writes
 // this CTA's shared memory when it exits.
 __device__ __forceinline__ void barrier_drain(uint64_t *bar, uint32_t parity, uint64_t start) {
     while (!barrier_test(bar, parity))
         if (clock_ns() - start > kTensorWaitLimitNs) return;
+}
+
+// True in one lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t elected;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(elected));
+    return elected != 0;
 }
 
 // ---------------------------------------------------------------- clusters
@@ -99,8 +126,11 @@ __device__ __forceinline__ float4 cluster_load(uint32_t address) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
     return v;
 }
+// Arrives in another CTA of the cluster, for what this CTA has read from tensor memory: there is no global or shared
+// memory to publish, and a release at cluster scope would wait for every load in flight (860 instead of 490 us for the
+// e4m3 product of 4608 x 15360 x 6144, once per block of 128 channels).
 __device__ __forceinline__ void barrier_arrive_at(uint32_t address) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(address) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(address) : "memory");
 }
 
 // ---------------------------------------------------------------- tile loads
@@ -176,6 +206,14 @@ __device__ __forceinline__ void tensor_load_32(uint32_t address, float *r) {
           "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]),
           "=r"(u[31])
         : "r"(address));
+}
+// 16 lanes x 16 columns in the fragment order: r[4 j + 0], r[4 j + 1] are columns 8 j + 2 (lane % 4) and the one after it of
+// lane base + lane / 4, r[4 j + 2], r[4 j + 3] the same columns eight lanes below.  A thread meets a quarter of the columns.
+__device__ __forceinline__ void tensor_load_fragment(uint32_t address, float *r) {
+    uint32_t *u = reinterpret_cast<uint32_t *>(r);
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "r"(address));
 }
 __device__ __forceinline__ void tensor_store_32(uint32_t address, const uint32_t *u) {
     asm volatile(
