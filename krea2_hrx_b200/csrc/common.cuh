@@ -37,8 +37,9 @@ int prepare_gemm_device();
 // Defined with the attention kernel: the same for it, and its share of the device status word.
 int prepare_attention_device();
 int take_attention_status(int *value);
-// Defined with the e4m3 product: its share of the status word.
+// Defined with the e4m3 product and the cross attention: their shares of the status word.
 int take_product_status(int *value);
+int take_cross_status(int *value);
 // Defined with the prologues: their first-use work, for callers about to capture a stream; and
 // prepare_gated_i8 whose attention rows have a pitch of their own (in elements).
 int prepare_prologue_device(cudaStream_t stream);

@@ -3,65 +3,523 @@
 // mask, bf16 and f16, heads of 8 to 128 channels, rows at any 16-byte pitch.
 //   out[b][i][h] = sum_j p_j v[b][j][h'] / sum_j p_j,  p_j = exp(scale q[b][i][h] . k[b][j][h'])
 // over the keys j < kv_lengths[b] whose mask byte is not zero, h' = h / (q_heads / kv_heads); zero where there is none.
+//
+// One pass over the keys with a running maximum and sum.  A CTA owns 128 rows of one key head: the query heads that share
+// it are packed (row r is query r / shares, head r % shares of the key head's), so a single query fills as many rows as
+// heads share its keys.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with f32 accumulators in tensor memory; K and V
+// tiles of 128 keys arrive by TMA as they lie (V is the second product's B operand with its channels innermost, so nothing
+// is transposed), a thread owns one row's softmax and writes P over S in tensor memory.  Two CTAs share an SM: one's
+// softmax, its start and its output run under the other's products.
+// Where the rows do not fill the device, a cluster of up to eight CTAs splits the keys of a row tile and adds its partial
+// outputs over distributed shared memory in the order of their rank: no workspace, the same bits every time.
+#include <atomic>
 #include <cmath>
 
-#include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace krea2 {
 namespace {
 
+__device__ int g_cross_status = 0;  // folded into krea2_device_status by take_cross_status
+constexpr int kCrossTimedOut = 128;
+
+constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
+
 struct CrossArgs {
-    const uint16_t *q, *k, *v;
+    const uint16_t *q;
     const int32_t *kv_lengths;
     const uint8_t *key_mask;
     uint16_t *out;
-    uint32_t q_len, kv_len, q_heads, shares, head_dim;
-    size_t q_batch_stride, q_stride, k_batch_stride, k_stride, v_batch_stride, v_stride, out_batch_stride, out_stride, mask_stride;
-    float scale_log2;
+    uint32_t rows, kv_len, shares, head_dim;  // rows: queries times shares
+    size_t q_batch_stride, q_stride, out_batch_stride, out_stride, mask_stride;
+    uint32_t k_batches, v_batches;  // 1 where every item of the batch shares its keys (values), 0 otherwise
+    float scale_log2;               // softmax scale times log2(e)
 };
 
-// A warp per query row and head, four channels per lane, one pass over the keys with the running maximum and sum.
+// kD: channels of a head as the tiles hold them, 64 or 128; those past head_dim are zero.
+template <int kD>
+struct Cross {
+    static constexpr int kSoftmaxWarps = 4, kLoadWarp = 4, kProductWarp = 5, kValueWarp = 6;
+    static constexpr int kThreads = 7 * 32;
+    static constexpr int kSubtileBytes = kRows * 128;  // 128 rows of 64 channels: one 128-byte swizzled column block
+    static constexpr int kTileBytes = kD / 64 * kSubtileBytes;
+    static constexpr int kStages = kD == 64 ? 2 : 1;
+    static constexpr int kTensorColumns = 256;  // S (then P) at 0, O at 128
+    static constexpr int kBarrierBytes = 256, kStatsBytes = kRows * 8;
+    static constexpr int kSharedBytes = (1 + 2 * kStages) * kTileBytes + 1024 + kBarrierBytes + kStatsBytes;
+    static_assert(2 * kStages * kTileBytes >= kRows * kD * 4, "the partial outputs take the place of keys and values");
+    static_assert(2 * (kSharedBytes + 1024) <= 228 * 1024 && 3 * kSharedBytes > 228 * 1024, "two CTAs share an SM and its tensor memory");
+};
+
 template <bool kBf16>
-__global__ void __launch_bounds__(256)
-cross_attention_kernel(const CrossArgs g) {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (item >= static_cast<uint64_t>(g.q_len) * g.q_heads) return;
-    const uint32_t batch = blockIdx.y, row = static_cast<uint32_t>(item / g.q_heads), head = static_cast<uint32_t>(item % g.q_heads);
-    const uint32_t kv_head = head / g.shares;
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if constexpr (kBf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The largest of three; a NaN among them stays one, so that a row that meets a NaN becomes NaN through its maximum.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// kind::f16: f32 accumulate (1 at bit 4), A and B f16 (0) or bf16 (1) at bits 7 and 10, B with its N side innermost at bit
+// 16, N/8 at bit 17, M/16 at bit 24.
+template <bool kBf16>
+__device__ constexpr uint32_t attention_descriptor(int n, bool n_inner) {
+    return (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (n_inner ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(kRows >> 4) << 24);
+}
+// A tile whose N side is innermost: rows of 64 channels (128 bytes, swizzled), eight rows of K to the next 1024 bytes, the
+// next 64 channels one subtile on.
+__device__ __forceinline__ uint64_t value_descriptor(uint32_t address, uint32_t subtile_bytes) {
+    return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(subtile_bytes >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void issue_f16(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+// A from tensor memory: 128 lanes of 16-bit pairs, eight columns per K = 16.
+__device__ __forceinline__ void issue_f16_tensor_a(uint32_t tmem, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem), "r"(a), "l"(b),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+template <int kD, bool kBf16>
+__global__ void __launch_bounds__(Cross<kD>::kThreads, 2)
+cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const CrossArgs g) {
+    using T = Cross<kD>;
+    extern __shared__ uint8_t shared_raw[];
+    uint8_t *q_tile = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *k_tiles = q_tile + T::kTileBytes, *v_tiles = k_tiles + T::kStages * T::kTileBytes;
+    uint64_t *q_full = reinterpret_cast<uint64_t *>(v_tiles + T::kStages * T::kTileBytes);
+    uint64_t *k_full = q_full + 1, *k_empty = k_full + T::kStages, *v_full = k_empty + T::kStages, *v_empty = v_full + T::kStages;
+    uint64_t *v_ready = v_empty + T::kStages, *s_full = v_ready + T::kStages, *p_full = s_full + 1, *o_full = p_full + 1, *words_full = o_full + 1;
+    uint32_t *words = reinterpret_cast<uint32_t *>(words_full + 2);  // [2][4]: which keys of a tile count, two tiles in turn
+    uint32_t *tmem_slot = words + 8;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    float *stats = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(q_full) + T::kBarrierBytes);  // [128][2]: reference and sum of a row
+    float *partial = reinterpret_cast<float *>(k_tiles);                                              // [128][kD], once the products are done
+    const Abort abort = {abort_flag, &g_cross_status, kCrossTimedOut};
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t parts = cluster_size(), rank = cluster_rank();
+    const uint32_t row0 = blockIdx.x / parts * kRows, kv_head = blockIdx.y, batch = blockIdx.z;
     int32_t length = static_cast<int32_t>(g.kv_len);
     if (g.kv_lengths) length = min(max(g.kv_lengths[batch], 0), length);
-    const uint16_t *q = g.q + batch * g.q_batch_stride + row * g.q_stride + head * g.head_dim;
-    float query[4], out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 4; i++) query[i] = lane + 32 * i < g.head_dim ? value_of<kBf16>(q[lane + 32 * i]) * g.scale_log2 : 0.0f;
-    float top = -INFINITY, sum = 0.0f;
-    for (int32_t j = 0; j < length; j++) {
-        if (g.key_mask && g.key_mask[batch * g.mask_stride + j] == 0) continue;
-        const uint16_t *k = g.k + batch * g.k_batch_stride + j * g.k_stride + kv_head * g.head_dim;
-        const uint16_t *v = g.v + batch * g.v_batch_stride + j * g.v_stride + kv_head * g.head_dim;
-        float score = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < g.head_dim) score = fmaf(query[i], value_of<kBf16>(k[lane + 32 * i]), score);
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) score += __shfl_xor_sync(0xffffffffu, score, off);
-        const float next = fmaxf(top, score), shift = next == -INFINITY ? 0.0f : next;
-        const float keep = exp2f(top - shift), p = exp2f(score - shift);
-        top = next;
-        sum = sum * keep + p;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < g.head_dim) out[i] = fmaf(p, value_of<kBf16>(v[lane + 32 * i]), out[i] * keep);
+    const uint32_t keys = static_cast<uint32_t>(length), tiles = (keys + kRows - 1) / kRows;
+    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * rank / parts);
+    const uint32_t last = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (rank + 1) / parts);
+    const uint32_t count = last - first;
+    uint32_t issued = 0;  // loader warps: tiles requested
+
+    if (threadIdx.x == 0) {
+        barrier_init(q_full, T::kSoftmaxWarps);
+        for (int s = 0; s < T::kStages; s++) {
+            barrier_init(k_full + s, 1);
+            barrier_init(k_empty + s, 1);
+            barrier_init(v_full + s, 1);
+            barrier_init(v_empty + s, 1);
+            barrier_init(v_ready + s, 1);
+        }
+        barrier_init(s_full, 1);
+        barrier_init(p_full, T::kSoftmaxWarps);
+        barrier_init(o_full, 1);
+        barrier_init(words_full, 1);
+        barrier_init(words_full + 1, 1);
+        *abort_flag = 0;
+        barrier_init_done();
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t *dst = g.out + batch * g.out_batch_stride + row * g.out_stride + head * g.head_dim;
+    if (warp == T::kProductWarp) {
+        __syncwarp();
+        tensor_alloc<1>(tmem_slot, T::kTensorColumns);
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    float reference = -INFINITY, sum = 0.0f;  // a softmax thread's row, in units of log2
+    bool alive = true;
+
+    if (warp == T::kLoadWarp) {
+        const bool elected = elect_lane();
+        for (uint32_t i = 0; i < count; i++, issued++) {
+            const uint32_t s = i % T::kStages;
+            if (!barrier_wait_warp(k_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
+            if (elected) {
+                barrier_expect(k_full + s, T::kTileBytes);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (lane + 32 * i < g.head_dim) dst[lane + 32 * i] = bits_of<kBf16>(out[i] * inverse);
+                for (int sub = 0; sub < kD / 64; sub++)
+                    load_tile_4d(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes, &map_k, k_full + s, sub * 64, static_cast<int>(kv_head),
+                                 static_cast<int>((first + i) * kRows), static_cast<int>(g.k_batches ? 0 : batch));
+            }
+            __syncwarp();
+        }
+    } else if (warp == T::kValueWarp) {
+        const bool elected = elect_lane();
+        for (uint32_t i = 0; i < count; i++, issued++) {
+            const uint32_t s = i % T::kStages, key0 = (first + i) * kRows;
+            uint32_t word[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const uint32_t key = key0 + w * 32 + lane;
+                word[w] = __ballot_sync(0xffffffffu, key < keys && (!g.key_mask || g.key_mask[batch * g.mask_stride + key] != 0));
+            }
+            if (!barrier_wait_warp(v_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
+            if (g.key_mask) {  // the tile that used these words two tiles ago has been through its second product
+                if (lane < 4) words[(i & 1u) * 4 + lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
+                __syncwarp();
+                if (lane == 0) barrier_arrive(words_full + (i & 1u));
+            }
+            uint8_t *tile = v_tiles + s * T::kTileBytes;
+            if (elected) {
+                barrier_expect(v_full + s, T::kTileBytes);
+#pragma unroll
+                for (int sub = 0; sub < kD / 64; sub++)
+                    load_tile_4d(tile + sub * T::kSubtileBytes, &map_v, v_full + s, sub * 64, static_cast<int>(kv_head), static_cast<int>(key0),
+                                 static_cast<int>(g.v_batches ? 0 : batch));
+            }
+            __syncwarp();
+            if (!g.key_mask && key0 + kRows <= keys) continue;
+            // Keys that do not count have the weight zero, but zero times what lies in their values may be NaN: their rows
+            // are cleared before the second product reads the tile.
+            if (!barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort)) break;
+            constexpr uint32_t kPieces = kD / 8;  // 16 bytes each
+#pragma unroll 1
+            for (uint32_t piece = lane; piece < kRows * kPieces; piece += 32) {
+                const uint32_t row = piece / kPieces, at = piece % kPieces;
+                const uint32_t bits = row < 32 ? word[0] : row < 64 ? word[1] : row < 96 ? word[2] : word[3];
+                if (!((bits >> (row & 31u)) & 1u))
+                    *reinterpret_cast<uint4 *>(tile + (at >> 3) * T::kSubtileBytes + row * 128 + (at & 7u) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) barrier_arrive(v_ready + s);
+        }
+    } else if (warp == T::kProductWarp) {
+        const bool elected = elect_lane();
+        constexpr uint32_t scores_idesc = attention_descriptor<kBf16>(kRows, false), values_idesc = attention_descriptor<kBf16>(kD, true);
+        if (count) alive = barrier_wait_warp(q_full, 0, abort);
+        // The pipe runs one thread's products in issue order and a commit covers all that was issued before it: the scores of
+        // a tile overwrite the weights of the one before only after the second product has read them, and the softmax that
+        // sees new scores may rescale O.
+        auto scores = [&](uint32_t i) {
+            const uint32_t s = i % T::kStages;
+            if (!barrier_wait_warp(k_full + s, (i / T::kStages) & 1u, abort)) return false;
+            tensor_fence_after();
+            if (elected) {
+#pragma unroll
+                for (int sub = 0; sub < kD / 64; sub++) {
+                    const uint64_t a = operand_descriptor(smem_address(q_tile + sub * T::kSubtileBytes));
+                    const uint64_t b = operand_descriptor(smem_address(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) issue_f16(tmem, a + 2 * k, b + 2 * k, scores_idesc, sub != 0 || k != 0);
+                }
+                tensor_commit(s_full);
+                tensor_commit(k_empty + s);
+            }
+            __syncwarp();
+            return true;
+        };
+        if (count && alive) alive = scores(0);
+        for (uint32_t i = 0; alive && i < count; i++) {
+            const uint32_t s = i % T::kStages;
+            const bool cleared = g.key_mask || (first + i + 1) * kRows > keys;
+            alive = cleared ? barrier_wait_warp(v_ready + s, g.key_mask ? (i / T::kStages) & 1u : 0u, abort)
+                            : barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort);
+            alive = alive && barrier_wait_warp(p_full, i & 1u, abort);
+            if (!alive) break;
+            tensor_fence_after();
+            if (elected) {
+                const uint64_t v = value_descriptor(smem_address(v_tiles + s * T::kTileBytes), T::kSubtileBytes);
+#pragma unroll
+                for (int k = 0; k < kRows / 16; k++) issue_f16_tensor_a(tmem + kRows, tmem + 8 * k, v + 128 * k, values_idesc, i != 0 || k != 0);
+                tensor_commit(v_empty + s);
+                if (i + 1 == count) tensor_commit(o_full);
+            }
+            __syncwarp();
+            if (i + 1 < count) alive = scores(i + 1);
+        }
+    } else {
+        // ---- softmax: thread = row
+        if (count) {
+            // The warp's 32 rows of Q, 16 bytes a piece, into the swizzled layout; what is past the rows or the head is zero.
+            constexpr uint32_t kPieces = kD / 8;
+#pragma unroll 4
+            for (uint32_t piece = lane; piece < 32 * kPieces; piece += 32) {
+                const uint32_t local = warp * 32 + piece / kPieces, at = piece % kPieces, row = row0 + local;
+                const bool inside = row < g.rows && at * 8 < g.head_dim;
+                const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
+                const uint16_t *from = g.q + (inside ? batch * g.q_batch_stride + query * g.q_stride + static_cast<size_t>(head) * g.head_dim + at * 8 : 0);
+                const uint32_t to = smem_address(q_tile + (at >> 3) * T::kSubtileBytes + local * 128 + (((at & 7u) ^ (local & 7u)) * 16));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(inside ? 16u : 0u) : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) barrier_arrive(q_full);
+        }
+        const uint32_t lane_bits = static_cast<uint32_t>(warp * 32) << 16;
+        const uint32_t s_at = tmem + lane_bits, o_at = tmem + kRows + lane_bits;
+        for (uint32_t i = 0; i < count; i++) {
+            uint32_t word[4];
+            const uint32_t key0 = (first + i) * kRows;
+            bool all = true;
+            if (g.key_mask) {
+                if (!(alive = barrier_wait_warp(words_full + (i & 1u), (i >> 1) & 1u, abort))) break;
+#pragma unroll
+                for (int w = 0; w < 4; w++) word[w] = words[(i & 1u) * 4 + w];
+                all = (word[0] & word[1] & word[2] & word[3]) == 0xffffffffu;
+            } else if (key0 + kRows > keys) {
+                all = false;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int32_t here = static_cast<int32_t>(keys - key0) - 32 * w;
+                    word[w] = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1u;
+                }
+            }
+            if (!(alive = barrier_wait_warp(s_full, i & 1u, abort))) break;
+            tensor_fence_after();
+            // The 128 scores pass through registers twice, 64 at a time: for the maximum and for the weights.
+            auto load_half = [&](int half, float (&v)[64]) {
+                tensor_load_32(s_at + half * 64, v);
+                tensor_load_32(s_at + half * 64 + 32, v + 32);
+                tensor_loads_done();
+                if (!all) {
+#pragma unroll
+                    for (int k = 0; k < 64; k++)
+                        if (!((word[2 * half + (k >> 5)] >> (k & 31)) & 1u)) v[k] = -INFINITY;
+                }
+            };
+            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                float v[64];
+                load_half(half, v);
+#pragma unroll
+                for (int k = 0; k < 64; k += 8)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) part[t] = max3_nan(part[t], v[k + t], v[k + 4 + t]);
+            }
+            const float top = max_nan(max3_nan(part[0], part[1], part[2]), part[3]) * g.scale_log2;
+            // The exponents' reference moves only when the maximum has grown by more than 2^8 (a weight of 256 is exact
+            // enough in either type, and neither O nor the sum changes its ratio); a NaN moves it for good.
+            float alpha = 1.0f;
+            const bool move = !(top <= reference + 8.0f);
+            if (move) {
+                alpha = exp2_approx(reference - top);
+                reference = top;
+                sum *= alpha;
+            }
+            if (i > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                for (int c = 0; c < kD; c += 32) {
+                    float o[32];
+                    tensor_load_32(o_at + c, o);
+                    tensor_loads_done();
+#pragma unroll
+                    for (int k = 0; k < 32; k++) o[k] *= alpha;
+                    tensor_store_32(o_at + c, reinterpret_cast<const uint32_t *>(o));
+                }
+                tensor_stores_done();
+            }
+            const float shift = reference == -INFINITY ? 0.0f : -reference;  // nothing counted yet: the weights are zero, not NaN
+            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                float v[64];
+                load_half(half, v);
+                uint32_t packed[32];
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    const float2 x = fma_pair(make_float2(v[k], v[k + 1]), make_float2(g.scale_log2, g.scale_log2), make_float2(shift, shift));
+                    const float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
+                    total[(k >> 1) & 3] += p0 + p1;
+                    packed[k / 2] = pack_pair<kBf16>(p0, p1);
+                }
+                tensor_store_32(s_at + half * 32, packed);
+            }
+            sum += (total[0] + total[1]) + (total[2] + total[3]);
+            tensor_stores_done();
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(p_full);
+        }
+        alive = alive && (count == 0 || barrier_wait_warp(o_full, 0, abort));
+        tensor_fence_after();
+        if (alive && parts == 1) {
+            // Through the warp's own rows of the Q tile (no product reads it any more), so that rows leave in pieces of 128 bytes.
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const uint32_t local = warp * 32 + lane;
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 32) {
+                float o[32];
+                if (count) {
+                    tensor_load_32(o_at + c, o);
+                    tensor_loads_done();
+                }
+#pragma unroll
+                for (int k = 0; k < 32; k += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[j] = count ? pack_pair<kBf16>(o[k + 2 * j] * inverse, o[k + 2 * j + 1] * inverse) : 0u;
+                    const uint32_t at = (c + k) / 8;
+                    *reinterpret_cast<uint4 *>(q_tile + (at >> 3) * T::kSubtileBytes + local * 128 + (((at & 7u) ^ (local & 7u)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            __syncwarp();
+            constexpr uint32_t kPieces = kD / 8;
+#pragma unroll 4
+            for (uint32_t piece = lane; piece < 32 * kPieces; piece += 32) {
+                const uint32_t mine = warp * 32 + piece / kPieces, at = piece % kPieces, row = row0 + mine;
+                if (row >= g.rows || at * 8 >= g.head_dim) continue;
+                const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
+                *reinterpret_cast<uint4 *>(g.out + batch * g.out_batch_stride + query * g.out_stride + static_cast<size_t>(head) * g.head_dim + at * 8) =
+                    *reinterpret_cast<const uint4 *>(q_tile + (at >> 3) * T::kSubtileBytes + mine * 128 + (((at & 7u) ^ (mine & 7u)) * 16));
+            }
+        } else if (alive && row0 + warp * 32 < g.rows) {
+            // A share of the keys: the row's reference, sum and unscaled output for the others to read.
+            const uint32_t local = warp * 32 + lane;
+            stats[2 * local] = reference;
+            stats[2 * local + 1] = sum;
+#pragma unroll 1
+            for (int c = 0; c < kD; c += 32) {
+                float o[32];
+                if (count) {
+                    tensor_load_32(o_at + c, o);
+                    tensor_loads_done();
+                }
+#pragma unroll
+                for (int k = 0; k < 32; k += 4)
+                    *reinterpret_cast<float4 *>(partial + local * kD + (((c + k) / 4) ^ (local & 7u)) * 4) =
+                        count ? make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+    }
+
+    tensor_fence_before();
+    __syncthreads();  // every role is done: the abort flag is final
+    tensor_fence_after();
+    if (*abort_flag && (warp == T::kLoadWarp || warp == T::kValueWarp) && lane == 0) {
+        uint64_t *full = warp == T::kLoadWarp ? k_full : v_full;
+        const uint64_t start = clock_ns();
+        for (uint32_t i = issued > T::kStages ? issued - T::kStages : 0u; i < issued; i++) barrier_drain(full + i % T::kStages, (i / T::kStages) & 1u, start);
+    }
+    if (warp == T::kProductWarp) {
+        __syncwarp();
+        tensor_free<1>(tmem, T::kTensorColumns);
+    }
+    if (parts == 1) return;
+    cluster_barrier();  // every share of this row tile is in shared memory
+    const uint32_t rows_here = min(static_cast<uint32_t>(kRows), g.rows - row0), pieces = g.head_dim / 4;
+    for (uint32_t item = threadIdx.x * parts + rank; item < rows_here * pieces; item += T::kThreads * parts) {
+        const uint32_t local = item / pieces, at = item % pieces, row = row0 + local;
+        float references[8], top = -INFINITY, total = 0.0f;
+        float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f), share[8];
+        float sums[8];
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+            if (r >= parts) continue;
+            const float2 stat = cluster_load_pair(cluster_address(stats + 2 * local, r));
+            share[r] = cluster_load(cluster_address(partial + local * kD + (at ^ (local & 7u)) * 4, r));
+            references[r] = stat.x, sums[r] = stat.y;
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++)
+            if (r < parts) top = max_nan(top, references[r]);
+        const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+            if (r >= parts) continue;
+            const float weight = exp2_approx(references[r] - shift);
+            total += weight * sums[r];
+            value.x += weight * share[r].x, value.y += weight * share[r].y, value.z += weight * share[r].z, value.w += weight * share[r].w;
+        }
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
+        *reinterpret_cast<uint2 *>(g.out + batch * g.out_batch_stride + query * g.out_stride + static_cast<size_t>(head) * g.head_dim + at * 4) =
+            make_uint2(pack_pair<kBf16>(value.x * inverse, value.y * inverse), pack_pair<kBf16>(value.z * inverse, value.w * inverse));
+    }
+    cluster_barrier();  // the others have read this CTA's share
+}
+
+// ---------------------------------------------------------------- host side
+// Keys or values [batch][kv_len][heads][head_dim] as boxes of 64 channels of one head x 128 rows.
+int states_map(CUtensorMap *map, bool bf16, const void *base, size_t head_dim, size_t heads, size_t rows, size_t batch, size_t stride, size_t batch_stride) {
+    const cuuint64_t dims[4] = {head_dim, heads, rows, batch};
+    const cuuint64_t strides[3] = {head_dim * 2, stride * 2, batch > 1 ? batch_stride * 2 : stride * 2};
+    const cuuint32_t box[4] = {64, 1, kRows, 1};
+    return make_tensor_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box);
+}
+
+template <int kD, bool kBf16>
+int launch_cross(cudaStream_t stream, const CUtensorMap &map_k, const CUtensorMap &map_v, size_t batch, size_t kv_heads, const CrossArgs &g) {
+    using T = Cross<kD>;
+    static Prepared prepared;
+    static std::atomic<int> known[64][9];  // clusters of so many CTAs that a device holds at once
+    if (int status = prepare_kernel(prepared, cross_attention_kernel<kD, kBf16>, T::kSharedBytes)) return status;
+    int device = 0;
+    KREA2_CUDA(cudaGetDevice(&device));
+    cudaLaunchConfig_t config = {};
+    config.blockDim = dim3(T::kThreads);
+    config.dynamicSmemBytes = T::kSharedBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    const uint32_t row_tiles = (g.rows + kRows - 1) / kRows, key_tiles = (g.kv_len + kRows - 1) / kRows;
+    const size_t tiles = row_tiles * batch * kv_heads;
+    // The keys are split as far as all clusters stay resident; each share has a tile of keys at least.
+    uint32_t parts = 1;
+    for (uint32_t more = 2; more <= 8 && more <= key_tiles; more++) {
+        int clusters = known[device][more].load(std::memory_order_relaxed);
+        if (clusters == 0) {
+            config.gridDim = dim3(more, 1, 1);
+            attribute.val.clusterDim.x = more;
+            KREA2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, cross_attention_kernel<kD, kBf16>, &config));
+            if (clusters < 1) clusters = 1;
+            known[device][more].store(clusters, std::memory_order_relaxed);
+        }
+        if (tiles > static_cast<size_t>(clusters)) break;
+        parts = more;
+    }
+    attribute.val.clusterDim.x = parts;
+    config.gridDim = dim3(row_tiles * parts, static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
+    const cudaError_t status = cudaLaunchKernelEx(&config, cross_attention_kernel<kD, kBf16>, map_k, map_v, g);
+    if (status != cudaSuccess) return fail(KREA2_RUNTIME, "cross_attention launch failed: %s", cudaGetErrorString(status));
+    return KREA2_OK;
 }
 
 }  // namespace
+
+int take_cross_status(int *value) {
+    KREA2_CUDA(cudaMemcpyFromSymbol(value, g_cross_status, sizeof(int)));
+    if (*value != 0) {
+        const int zero = 0;
+        KREA2_CUDA(cudaMemcpyToSymbol(g_cross_status, &zero, sizeof(int)));
+    }
+    return KREA2_OK;
+}
+
 }  // namespace krea2
 
 using namespace krea2;
@@ -92,17 +550,20 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
     KREA2_REQUIRE(q && out && (kv_len == 0 || (k && v)), "%s: null buffer", name);
     KREA2_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "%s: buffers must be 16-byte aligned", name);
     KREA2_REQUIRE(reinterpret_cast<uintptr_t>(kv_lengths) % 4 == 0, "%s: kv_lengths must be 4-byte aligned", name);
-    const CrossArgs g = {static_cast<const uint16_t *>(q), static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), kv_lengths, static_cast<const uint8_t *>(key_mask),
-                         static_cast<uint16_t *>(out), static_cast<uint32_t>(q_len), static_cast<uint32_t>(kv_len), static_cast<uint32_t>(q_heads),
-                         static_cast<uint32_t>(q_heads / kv_heads), static_cast<uint32_t>(head_dim), q_batch_stride, q_stride, k_batch_stride,
-                         k_stride, v_batch_stride, v_stride, out_batch_stride, out_stride, mask_stride, scale * 1.44269504088896340736f};
-    const size_t blocks = (q_len * q_heads + 7) / 8;
-    KREA2_REQUIRE(blocks <= 0x7fffffff, "%s: %zu query rows of %zu heads exceed the grid", name, q_len, q_heads);
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(batch));
+    const size_t shares = q_heads / kv_heads;
+    KREA2_REQUIRE(q_len * shares <= 0x7fffff00 / 8, "%s: %zu queries of %zu heads to a key head exceed the grid", name, q_len, shares);
+    const bool bf16 = kind == KREA2_BF16, k_shared = batch > 1 && k_batch_stride == 0, v_shared = batch > 1 && v_batch_stride == 0;
+    const CrossArgs g = {static_cast<const uint16_t *>(q), kv_lengths, static_cast<const uint8_t *>(key_mask), static_cast<uint16_t *>(out),
+                         static_cast<uint32_t>(q_len * shares), static_cast<uint32_t>(kv_len), static_cast<uint32_t>(shares), static_cast<uint32_t>(head_dim),
+                         q_batch_stride, q_stride, out_batch_stride, out_stride, mask_stride, k_shared ? 1u : 0u, v_shared ? 1u : 0u,
+                         scale * 1.44269504088896340736f};
+    CUtensorMap map_k = {}, map_v = {};  // without keys no load is issued
+    if (kv_len != 0) {
+        if (int status = states_map(&map_k, bf16, k, head_dim, kv_heads, kv_len, k_shared ? 1 : batch, k_stride, k_batch_stride)) return status;
+        if (int status = states_map(&map_v, bf16, v, head_dim, kv_heads, kv_len, v_shared ? 1 : batch, v_stride, v_batch_stride)) return status;
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (kind == KREA2_BF16) cross_attention_kernel<true><<<grid, 256, 0, s>>>(g);
-    else cross_attention_kernel<false><<<grid, 256, 0, s>>>(g);
-    const cudaError_t status = cudaGetLastError();
-    if (status != cudaSuccess) return fail(KREA2_RUNTIME, "%s launch failed: %s", name, cudaGetErrorString(status));
-    return KREA2_OK;
+    if (head_dim <= 64)
+        return bf16 ? launch_cross<64, true>(s, map_k, map_v, batch, kv_heads, g) : launch_cross<64, false>(s, map_k, map_v, batch, kv_heads, g);
+    return bf16 ? launch_cross<128, true>(s, map_k, map_v, batch, kv_heads, g) : launch_cross<128, false>(s, map_k, map_v, batch, kv_heads, g);
 }

@@ -1471,9 +1471,10 @@ extern "C" int krea2_device_status(int *host_status) {
         int zero = 0;
         KREA2_CUDA(cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)));
     }
-    int attention = 0, product = 0;
+    int attention = 0, product = 0, cross = 0;
     if (int status = take_attention_status(&attention)) return status;
     if (int status = take_product_status(&product)) return status;
-    *host_status = value | attention | product;
+    if (int status = take_cross_status(&cross)) return status;
+    *host_status = value | attention | product | cross;
     return KREA2_OK;
 }

@@ -108,6 +108,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
 // The shared::cluster address of `p` (in this CTA's shared memory) inside CTA `rank`.
 __device__ __forceinline__ uint32_t cluster_address(const void *p, uint32_t rank) {
     uint32_t out;
@@ -124,6 +129,11 @@ __device__ __forceinline__ void cluster_store(uint32_t address, uint32_t value) 
 __device__ __forceinline__ float4 cluster_load(uint32_t address) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 cluster_load_pair(uint32_t address) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(address) : "memory");
     return v;
 }
 // Arrives in another CTA of the cluster, for what this CTA has read from tensor memory: there is no global or shared
