@@ -3,7 +3,9 @@
 //   krea2_prepare_plain_fp8  the codes of rows as they are
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include <atomic>
+
+#include "tensor_core.cuh"
 
 namespace krea2 {
 namespace {
@@ -23,24 +25,55 @@ struct PrepareArgs {
     float eps, weight_offset;
 };
 
-// Eight consecutive channels from `at` of one row: one 16-byte access where rows are aligned to it, single
-// elements (zero past the row's end) otherwise.
+// The channels of a thread's run of eight.  Where rows are aligned they are neighbours, moved by one 16-byte access, and
+// sixteen lanes own a scale's group; otherwise they lie 32 apart, so that a warp's single-element accesses are contiguous,
+// and all lanes own half of two groups.
 template <bool kVector>
-__device__ __forceinline__ void load8(const uint16_t *row, uint32_t at, uint32_t width, uint16_t (&v)[8]) {
+__device__ __forceinline__ uint32_t channel_of(uint32_t run, int i) {
+    return kVector ? run * 8 + i : (run & ~31u) * 8 + i * 32 + (run & 31u);
+}
+template <bool kVector>
+__device__ __forceinline__ uint4 load8(const uint16_t *row, uint32_t run, uint32_t width) {
     if constexpr (kVector) {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(row + at);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[2 * i] = static_cast<uint16_t>(w[i]), v[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+        return run * 8 < width ? *reinterpret_cast<const uint4 *>(row + run * 8) : make_uint4(0, 0, 0, 0);
     } else {
+        uint32_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = at + i < width ? row[at + i] : uint16_t(0);
+        for (int i = 0; i < 8; i++) {
+            const uint32_t at = channel_of<false>(run, i);
+            v[i] = at < width ? row[at] : 0u;
+        }
+        return make_uint4(v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16), v[6] | (v[7] << 16));
+    }
+}
+template <bool kVector>
+__device__ __forceinline__ void store8(uint16_t *row, uint32_t run, uint32_t width, uint4 v) {
+    if constexpr (kVector) {
+        if (run * 8 < width) *reinterpret_cast<uint4 *>(row + run * 8) = v;
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t at = channel_of<false>(run, i);
+            if (at < width) row[at] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+}
+template <bool kBf16>
+__device__ __forceinline__ void unpack8(uint4 raw, float (&v)[8]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[2 * i] = value_of<kBf16>(static_cast<uint16_t>(w[i]));
+        v[2 * i + 1] = value_of<kBf16>(static_cast<uint16_t>(w[i] >> 16));
     }
 }
 
+// The sum over the block; `shared` [32] may be used again two calls later.
 __device__ __forceinline__ float block_sum(float v, float *shared) {
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    if (blockDim.x == 32) return v;
     if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
     v = (threadIdx.x & 31) < (blockDim.x >> 5) ? shared[threadIdx.x & 31] : 0.0f;
@@ -49,98 +82,157 @@ __device__ __forceinline__ float block_sum(float v, float *shared) {
     return v;
 }
 
-// One block per row.  A thread owns kPer runs of eight channels, blockDim.x runs apart, so sixteen neighbouring
-// lanes own one scale's group; the row stays in registers between the sum of squares and the codes.
-template <bool kBf16, bool kNorm, bool kVector, int kPer>
-__global__ void __launch_bounds__(1024)
+// A thread owns kPer runs of eight channels, blockDim.x runs apart; the row stays in registers between the sum of squares and
+// the codes.  HBM-bound: a block walks rows gridDim.x apart and requests the next one before it works on the present one
+// (not the widest rows, whose values fill the registers).
+template <bool kBf16, bool kNorm, bool kResidual, bool kVector, int kPer>
+__global__ void __launch_bounds__(kPer == 1 ? 1024 : kPer == 2 ? 256 : 512, kPer == 2 ? 3 : 1)
 prepare_fp8_kernel(const PrepareArgs g) {
-    __shared__ float partial[32];
-    const size_t row = blockIdx.x;
-    const uint16_t *x = g.x + row * g.x_stride;
-    float v[kPer][8];
-    float squares = 0.0f;
+    constexpr bool kAhead = kVector && kPer <= 4;  // single elements are packed as they arrive: asking early would wait for them
+    __shared__ float partial[2][32];
+    const bool wide_weight = kVector && (reinterpret_cast<uintptr_t>(g.weight) & 15u) == 0u;
+    uint4 x[kPer], residual[kResidual ? kPer : 1];
+    auto run_of = [&](int j) { return threadIdx.x + j * blockDim.x; };
+    auto request = [&](size_t row) {
 #pragma unroll
-    for (int j = 0; j < kPer; j++) {
-        const uint32_t at = (threadIdx.x + j * blockDim.x) * 8;
+        for (int j = 0; j < kPer; j++) {
+            x[j] = load8<kVector>(g.x + row * g.x_stride, run_of(j), g.width);
+            if constexpr (kResidual) residual[j] = load8<kVector>(g.residual + row * g.residual_stride, run_of(j), g.width);
+        }
+    };
+    if (kAhead) request(blockIdx.x);
+    for (size_t row = blockIdx.x, count = 0; row < g.tokens; row += gridDim.x, count++) {
+        if (!kAhead) request(row);
+        float v[kPer][8];
+        float squares = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[j][i] = 0.0f;
-        if (at >= g.width) continue;
-        uint16_t raw[8];
-        load8<kVector>(x, at, g.width, raw);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[j][i] = value_of<kBf16>(raw[i]);
-        if constexpr (kNorm) {
-            if (g.residual != nullptr) {
-                uint16_t other[8];
-                load8<kVector>(g.residual + row * g.residual_stride, at, g.width, other);
+        for (int j = 0; j < kPer; j++) {
+            unpack8<kBf16>(x[j], v[j]);
+            if constexpr (kResidual) {
                 // The next layer reads the sum rounded to the stream's type, so the norm is taken of that.
+                float other[8];
+                unpack8<kBf16>(residual[j], other);
+                uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    raw[i] = bits_of<kBf16>(v[j][i] + value_of<kBf16>(other[i]));
-                    v[j][i] = value_of<kBf16>(raw[i]);
-                }
-                if (g.sum != nullptr) {
-                    uint16_t *sum = g.sum + row * g.sum_stride + at;
-                    if constexpr (kVector) {
-                        uint32_t w[4];
+                for (int i = 0; i < 4; i++)
+                    w[i] = bits_of<kBf16>(v[j][2 * i] + other[2 * i]) | (static_cast<uint32_t>(bits_of<kBf16>(v[j][2 * i + 1] + other[2 * i + 1])) << 16);
+                const uint4 total = make_uint4(w[0], w[1], w[2], w[3]);
+                unpack8<kBf16>(total, v[j]);
+                if (g.sum != nullptr) store8<kVector>(g.sum + row * g.sum_stride, run_of(j), g.width, total);
+            }
+            if constexpr (kNorm) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = raw[2 * i] | (static_cast<uint32_t>(raw[2 * i + 1]) << 16);
-                        *reinterpret_cast<uint4 *>(sum) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int i = 0; i < 8; i++) squares = fmaf(v[j][i], v[j][i], squares);
+            }
+        }
+        if (kAhead && row + gridDim.x < g.tokens) request(row + gridDim.x);
+        if constexpr (kNorm) {
+            const float rinv = 1.0f / sqrtf(block_sum(squares, partial[count & 1]) / static_cast<float>(g.width) + g.eps);
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                float weight[8] = {};
+                if (g.weight != nullptr) {
+                    if (wide_weight) {
+                        if (run_of(j) * 8 < g.width) {
+                            *reinterpret_cast<float4 *>(weight) = __ldg(reinterpret_cast<const float4 *>(g.weight + run_of(j) * 8));
+                            *reinterpret_cast<float4 *>(weight + 4) = __ldg(reinterpret_cast<const float4 *>(g.weight + run_of(j) * 8 + 4));
+                        }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            if (at + i < g.width) sum[i] = raw[i];
+                        for (int i = 0; i < 8; i++) {
+                            const uint32_t at = channel_of<kVector>(run_of(j), i);
+                            if (at < g.width) weight[i] = __ldg(g.weight + at);
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 8; i++) squares = fmaf(v[j][i], v[j][i], squares);
-        }
-    }
-    float rinv = 1.0f;
-    if constexpr (kNorm) rinv = 1.0f / sqrtf(block_sum(squares, partial) / static_cast<float>(g.width) + g.eps);
-#pragma unroll
-    for (int j = 0; j < kPer; j++) {
-        const uint32_t at = (threadIdx.x + j * blockDim.x) * 8;
-        if constexpr (kNorm) {
-            if (at < g.width) {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (kVector || at + i < g.width) v[j][i] = v[j][i] * rinv * (g.weight_offset + (g.weight ? g.weight[at + i] : 0.0f));
+                for (int i = 0; i < 8; i++) v[j][i] = v[j][i] * rinv * (g.weight_offset + weight[i]);
             }
         }
-        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[j][i]));
+        for (int j = 0; j < kPer; j++) {
+            const uint32_t run = run_of(j);
+            // What lies past the row's end was read as zero; a weight cannot make it more than that (a norm of such a zero
+            // may be NaN in a row that is, which no maximum shows).
+            float top[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        const float scale = fmaxf(top / kE4m3Max, kScaleFloor);
-        const float inverse = 1.0f / scale;
-        if (at >= g.width) continue;
-        uint8_t *q = g.q + row * g.out_stride + at;
-        uint32_t w[2];
+            for (int i = 0; i < 8; i++) top[kVector ? 0 : i >> 2] = fmaxf(top[kVector ? 0 : i >> 2], fabsf(v[j][i]));
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[j][4 * i] * inverse, v[j][4 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[j][4 * i + 2] * inverse, v[j][4 * i + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
-            w[i] = lo | (hi << 16);
+            for (int off = kVector ? 8 : 16; off >= 1; off >>= 1) {
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+                if constexpr (!kVector) top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+            }
+            float scale[2], inverse[2];
+#pragma unroll
+            for (int h = 0; h < (kVector ? 1 : 2); h++) {
+                scale[h] = fmaxf(__fdiv_rn(top[h], kE4m3Max), kScaleFloor);
+                inverse[h] = __frcp_rn(scale[h]);
+            }
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float by = inverse[kVector ? 0 : i];
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[j][4 * i] * by, v[j][4 * i + 1] * by), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[j][4 * i + 2] * by, v[j][4 * i + 3] * by), __NV_SATFINITE, __NV_E4M3);
+                w[i] = lo | (hi << 16);
+            }
+            uint8_t *q = g.q + row * g.out_stride;
+            if constexpr (kVector) {
+                if (run * 8 >= g.width) continue;
+                *reinterpret_cast<uint2 *>(q + run * 8) = make_uint2(w[0], w[1]);
+                if ((run & 15u) == 0u) g.q_scale[row * g.groups + run / 16] = scale[0];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t at = channel_of<false>(run, i);
+                    if (at < g.width) q[at] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
+                }
+                const uint32_t group = run / 32 * 2 + (run & 1u);
+                if ((run & 31u) < 2u && group < g.groups) g.q_scale[row * g.groups + group] = scale[run & 1u];
+            }
         }
-        if (at + 8 <= g.width) {
-            *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[1]);
-        } else {
-            for (uint32_t i = 0; at + i < g.width; i++) q[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
-        }
-        if (((at / 8) & 15) == 0) g.q_scale[row * g.groups + at / kGroup] = scale;
     }
 }
 
-template <bool kBf16, bool kNorm, bool kVector>
-void launch_prepare(cudaStream_t stream, const PrepareArgs &g) {
+template <bool kBf16, bool kNorm, bool kResidual, bool kVector, int kPer>
+int launch_runs(cudaStream_t stream, const PrepareArgs &g, uint32_t runs) {
+    static std::atomic<int> known[64][33];  // blocks of so many warps that an SM holds
+    const uint32_t threads = ((runs + kPer - 1) / kPer + 31) / 32 * 32;
+    int device = 0;
+    KREA2_CUDA(cudaGetDevice(&device));
+    if (device < 0 || device >= 64) return fail(KREA2_INTERNAL, "device index %d out of range", device);
+    int blocks = known[device][threads / 32].load(std::memory_order_relaxed);
+    if (blocks == 0) {
+        KREA2_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, prepare_fp8_kernel<kBf16, kNorm, kResidual, kVector, kPer>,
+                                                                 static_cast<int>(threads), 0));
+        if (blocks < 1) blocks = 1;
+        known[device][threads / 32].store(blocks, std::memory_order_relaxed);
+    }
+    const uint32_t resident = static_cast<uint32_t>(blocks) * static_cast<uint32_t>(multiprocessors());
+    prepare_fp8_kernel<kBf16, kNorm, kResidual, kVector, kPer><<<g.tokens < resident ? g.tokens : resident, threads, 0, stream>>>(g);
+    return KREA2_OK;
+}
+
+// Few rows: one run a thread, for the latency (3.6 us for 148 rows of 6144).  Many: two to four, so that several blocks share
+// an SM and one's loads run under another's sums (4608 rows of 6144 and their residual take 70 us with one run a thread and
+// a block per row).
+template <bool kBf16, bool kNorm, bool kResidual, bool kVector>
+int launch_prepare(cudaStream_t stream, const PrepareArgs &g) {
     const uint32_t runs = (g.width + 7) / 8;
-    auto threads = [&](uint32_t per) { return ((runs + per - 1) / per + 31) / 32 * 32; };
-    if (runs <= 1024) prepare_fp8_kernel<kBf16, kNorm, kVector, 1><<<g.tokens, threads(1), 0, stream>>>(g);
-    else if (runs <= 2048) prepare_fp8_kernel<kBf16, kNorm, kVector, 2><<<g.tokens, threads(2), 0, stream>>>(g);
-    else prepare_fp8_kernel<kBf16, kNorm, kVector, 4><<<g.tokens, threads(4), 0, stream>>>(g);
+    if (runs <= 1024 && (!kVector || g.tokens <= static_cast<uint32_t>(multiprocessors()) || runs <= 128))
+        return launch_runs<kBf16, kNorm, kResidual, kVector, 1>(stream, g, runs);
+    if (runs <= 512) return launch_runs<kBf16, kNorm, kResidual, kVector, 2>(stream, g, runs);
+    if (runs <= 1536) return launch_runs<kBf16, kNorm, kResidual, kVector, 3>(stream, g, runs);
+    if (runs <= 2048) return launch_runs<kBf16, kNorm, kResidual, kVector, 4>(stream, g, runs);
+    return launch_runs<kBf16, kNorm, kResidual, kVector, 8>(stream, g, runs);
+}
+
+template <bool kBf16, bool kNorm>
+int launch_residual(cudaStream_t stream, const PrepareArgs &g, bool vector) {
+    if constexpr (kNorm) {
+        if (g.residual) return vector ? launch_prepare<kBf16, true, true, true>(stream, g) : launch_prepare<kBf16, true, true, false>(stream, g);
+    }
+    return vector ? launch_prepare<kBf16, kNorm, false, true>(stream, g) : launch_prepare<kBf16, kNorm, false, false>(stream, g);
 }
 
 template <bool kNorm>
@@ -148,8 +240,7 @@ int run_prepare(const char *name, cudaStream_t stream, const PrepareArgs &g, int
     const bool vector = g.width % 8 == 0 && g.x_stride % 8 == 0 && aligned16(g.x) &&
                         (!g.residual || (g.residual_stride % 8 == 0 && aligned16(g.residual))) &&
                         (!g.sum || (g.sum_stride % 8 == 0 && aligned16(g.sum)));
-    if (kind == KREA2_BF16) vector ? launch_prepare<true, kNorm, true>(stream, g) : launch_prepare<true, kNorm, false>(stream, g);
-    else vector ? launch_prepare<false, kNorm, true>(stream, g) : launch_prepare<false, kNorm, false>(stream, g);
+    if (int status = kind == KREA2_BF16 ? launch_residual<true, kNorm>(stream, g, vector) : launch_residual<false, kNorm>(stream, g, vector)) return status;
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "%s launch failed: %s", name, cudaGetErrorString(status));
     return KREA2_OK;

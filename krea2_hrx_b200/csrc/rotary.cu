@@ -5,7 +5,7 @@
 //   krea2_rotary              queries and keys turned, in place or into other buffers
 #include <cmath>
 
-#include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace krea2 {
 namespace {
@@ -20,6 +20,15 @@ struct RotaryArgs {
     float magnitude, direction;
 };
 
+__device__ __forceinline__ const uint16_t *head_in(const RotaryArgs &g, size_t token, uint32_t head) {
+    return head < g.q_heads ? g.q + token * g.q_stride + static_cast<size_t>(head) * g.head_dim
+                            : g.k + token * g.k_stride + static_cast<size_t>(head - g.q_heads) * g.head_dim;
+}
+__device__ __forceinline__ uint16_t *head_out(const RotaryArgs &g, size_t token, uint32_t head) {
+    return head < g.q_heads ? g.q_out + token * g.q_out_stride + static_cast<size_t>(head) * g.head_dim
+                            : g.k_out + token * g.k_out_stride + static_cast<size_t>(head - g.q_heads) * g.head_dim;
+}
+
 // cos and sin of position * frequency.  The product and its remainder by whole turns are taken in f64 (at position
 // 10^6 an f32 product is off by 0.06 radians), what is left is below half a turn and exact enough in f32.
 __device__ __forceinline__ void turn_of(int32_t position, double frequency, float &cosine, float &sine) {
@@ -27,37 +36,165 @@ __device__ __forceinline__ void turn_of(int32_t position, double frequency, floa
     sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sine, &cosine);
 }
 
-// One block per token: the token's cosines and sines go to shared memory, then its heads are turned pair by pair.
+template <bool kBf16>
+__device__ __forceinline__ float low_value(uint32_t word) { return value_of<kBf16>(static_cast<uint16_t>(word)); }
+template <bool kBf16>
+__device__ __forceinline__ float high_value(uint32_t word) { return value_of<kBf16>(static_cast<uint16_t>(word >> 16)); }
+template <bool kBf16>
+__device__ __forceinline__ uint32_t word_of(float lo, float hi) {
+    return bits_of<kBf16>(lo) | (static_cast<uint32_t>(bits_of<kBf16>(hi)) << 16);
+}
+
+// HBM-bound.  A warp walks heads of one token, four heads' loads in flight (the first are under way before the angles are
+// taken); `warps` warps share a token's heads where the tokens do not fill the device.  The token's cosines and sines are
+// taken once per warp, a pair per lane, and lie in shared memory; a lane keeps those of its piece in registers.
+constexpr int kBatch = 4;
+
+__device__ __forceinline__ void take_turns(const RotaryArgs &g, size_t token, uint32_t lane, float2 *turn) {
+    const int32_t position = g.positions ? g.positions[token] : static_cast<int32_t>(token);
+    for (uint32_t pair = lane; pair < g.half; pair += 32) {
+        float c, s;
+        turn_of(position, __ldg(g.frequencies + pair), c, s);
+        turn[pair] = make_float2(c * g.magnitude, s * g.magnitude * g.direction);
+    }
+    __syncwarp();
+}
+
+// Heads on 16-byte boundaries: a lane owns one piece of eight channels.  A piece of the half layout meets its partners, half
+// a rotary part away in the same head, by shuffles, so that every load and store of a warp is contiguous.
 template <bool kBf16, bool kInterleaved>
 __global__ void __launch_bounds__(256)
-rotary_kernel(const RotaryArgs g) {
-    __shared__ float cosines[256], sines[256];
-    const size_t token = blockIdx.x;
-    const int32_t position = g.positions ? g.positions[token] : static_cast<int32_t>(token);
-    for (uint32_t i = threadIdx.x; i < g.half; i += blockDim.x) {
-        float c, s;
-        turn_of(position, g.frequencies[i], c, s);
-        cosines[i] = c * g.magnitude;
-        sines[i] = s * g.magnitude * g.direction;
-    }
-    __syncthreads();
-    const uint32_t units = g.head_dim - g.half;  // pairs, then the channels that are not turned
-    const uint32_t count = (g.q_heads + g.kv_heads) * units;
-    for (uint32_t item = threadIdx.x; item < count; item += blockDim.x) {
-        const uint32_t head = item / units, unit = item % units;
-        const bool is_q = head < g.q_heads;
-        const uint16_t *in = is_q ? g.q + token * g.q_stride + head * g.head_dim : g.k + token * g.k_stride + (head - g.q_heads) * g.head_dim;
-        uint16_t *out = is_q ? g.q_out + token * g.q_out_stride + head * g.head_dim : g.k_out + token * g.k_out_stride + (head - g.q_heads) * g.head_dim;
-        if (unit < g.half) {
-            const uint32_t first = kInterleaved ? 2 * unit : unit, second = kInterleaved ? first + 1 : unit + g.half;
-            const float a = value_of<kBf16>(in[first]), b = value_of<kBf16>(in[second]);
-            const float c = cosines[unit], s = sines[unit];
-            out[first] = bits_of<kBf16>(a * c - b * s);
-            out[second] = bits_of<kBf16>(b * c + a * s);
-        } else {
-            out[unit + g.half] = in[unit + g.half];
+rotary_pieces_kernel(const RotaryArgs g, uint32_t tokens, uint32_t warps) {
+    __shared__ float2 turns_of_warp[8][256];
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const size_t token = item / warps;
+    if (token >= tokens) return;
+    const uint32_t share = static_cast<uint32_t>(item % warps), lane = threadIdx.x & 31;
+    const uint32_t pieces = g.head_dim / 8, heads = g.q_heads + g.kv_heads;
+    bool taken = false;
+    for (uint32_t piece0 = 0; piece0 < pieces; piece0 += 32) {
+        const uint32_t here = min(32u, pieces - piece0), per_pass = 32 / here;  // heads side by side in a warp
+        const uint32_t piece = piece0 + lane % here, offset = lane / here, stride = warps * per_pass;
+        const bool idle = offset >= per_pass;
+        uint4 x[kBatch];
+        auto request = [&](uint32_t head0) {
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const uint32_t head = head0 + offset + b * stride;
+                x[b] = make_uint4(0, 0, 0, 0);
+                if (!idle && head < heads) x[b] = *reinterpret_cast<const uint4 *>(head_in(g, token, head) + piece * 8);
+            }
+        };
+        request(share * per_pass);
+        float2 *turn = turns_of_warp[threadIdx.x >> 5];
+        if (!taken) take_turns(g, token, lane, turn);
+        taken = true;
+        constexpr int kPairs = kInterleaved ? 4 : 8;
+        const uint32_t away = kInterleaved ? 0u : g.half / 8;  // pieces to a piece's partner
+        const bool second = !kInterleaved && piece >= away;
+        const uint32_t pair0 = (second ? piece - away : piece) * kPairs;
+        const uint32_t inside = kInterleaved ? (g.half > pair0 ? min(4u, g.half - pair0) : 0u) : (piece < 2 * away ? 8u : 0u);  // pairs that turn
+        const uint32_t partner = second ? lane - away : lane + away;
+        float2 by[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; i++) {
+            by[i] = make_float2(1.0f, 0.0f);
+            if (i < inside) by[i] = turn[pair0 + i];
+            if (!kInterleaved && !second) by[i].y = -by[i].y;  // own * cos + partner * sin, the first of a pair against -sin
+        }
+        for (uint32_t head0 = share * per_pass; head0 < heads; head0 += kBatch * stride) {
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                uint32_t *own = reinterpret_cast<uint32_t *>(&x[b]);
+                if constexpr (kInterleaved) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float p = low_value<kBf16>(own[i]), q = high_value<kBf16>(own[i]);
+                        if (i < inside) own[i] = word_of<kBf16>(p * by[i].x - q * by[i].y, q * by[i].x + p * by[i].y);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t other = __shfl_sync(0xffffffffu, own[i], partner & 31u);
+                        const float2 c0 = by[2 * i], c1 = by[2 * i + 1];
+                        const uint32_t turned = word_of<kBf16>(low_value<kBf16>(own[i]) * c0.x + low_value<kBf16>(other) * c0.y,
+                                                               high_value<kBf16>(own[i]) * c1.x + high_value<kBf16>(other) * c1.y);
+                        if (inside) own[i] = turned;  // a channel that is not turned is copied, whatever it holds
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                const uint32_t head = head0 + offset + b * stride;
+                if (!idle && head < heads) *reinterpret_cast<uint4 *>(head_out(g, token, head) + piece * 8) = x[b];
+            }
+            if (head0 + kBatch * stride < heads) request(head0 + kBatch * stride);
         }
     }
+}
+
+// Other heads: a lane owns one pair; the channels from `copied` on, which are not turned and fall on 16-byte boundaries, are
+// copied in pieces, those between one by one.
+template <bool kBf16, bool kInterleaved>
+__global__ void __launch_bounds__(256)
+rotary_pairs_kernel(const RotaryArgs g, uint32_t tokens, uint32_t warps, uint32_t copied) {
+    __shared__ float2 turns_of_warp[8][256];
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const size_t token = item / warps;
+    if (token >= tokens) return;
+    const uint32_t share = static_cast<uint32_t>(item % warps), lane = threadIdx.x & 31;
+    float2 *turn = turns_of_warp[threadIdx.x >> 5];
+    take_turns(g, token, lane, turn);
+    const uint32_t heads = g.q_heads + g.kv_heads, units = copied - g.half;
+    for (uint32_t unit0 = 0; unit0 < units; unit0 += 32) {
+        const uint32_t here = min(32u, units - unit0), per_pass = 32 / here, stride = warps * per_pass;
+        const uint32_t unit = unit0 + lane % here, offset = lane / here;
+        if (offset >= per_pass) continue;
+        const bool turns = unit < g.half;
+        const float2 by = turns ? turn[unit] : make_float2(1.0f, 0.0f);
+        const uint32_t first = !turns ? unit + g.half : kInterleaved ? 2 * unit : unit;
+        const uint32_t second = !turns ? first : kInterleaved ? first + 1 : unit + g.half;
+        for (uint32_t head = share * per_pass + offset; head < heads; head += kBatch * stride) {
+            uint16_t a[kBatch], b[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) {
+                if (head + k * stride >= heads) break;
+                const uint16_t *in = head_in(g, token, head + k * stride);
+                a[k] = in[first], b[k] = in[second];
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; k++) {
+                if (head + k * stride >= heads) break;
+                uint16_t *out = head_out(g, token, head + k * stride);
+                if (turns) {
+                    const float x = value_of<kBf16>(a[k]), y = value_of<kBf16>(b[k]);
+                    out[second] = bits_of<kBf16>(y * by.x + x * by.y);
+                    out[first] = bits_of<kBf16>(x * by.x - y * by.y);
+                } else {
+                    out[first] = a[k];
+                }
+            }
+        }
+    }
+    const uint32_t pieces = (g.head_dim - copied) / 8;
+    for (uint32_t item8 = lane; item8 < heads * pieces; item8 += 32) {
+        const uint32_t head = item8 / pieces, at = copied + item8 % pieces * 8;
+        if (head % warps == share) *reinterpret_cast<uint4 *>(head_out(g, token, head) + at) = *reinterpret_cast<const uint4 *>(head_in(g, token, head) + at);
+    }
+}
+
+template <bool kBf16, bool kInterleaved>
+void launch_rotary(cudaStream_t stream, uint32_t tokens, const RotaryArgs &g, bool aligned) {
+    // Pieces need partners a whole number of pieces away, within the 32 pieces that a warp holds of a head.
+    const bool pieces = aligned && (kInterleaved || (g.half % 8 == 0 && g.head_dim <= 256));
+    const uint32_t copied = aligned ? (2 * g.half + 7) / 8 * 8 : g.head_dim;
+    const uint32_t units = min(32u, pieces ? g.head_dim / 8 : copied - g.half), per_pass = 32 / units;
+    // About 32 warps an SM, each with a pass over the heads at least.
+    const uint32_t passes = (g.q_heads + g.kv_heads + per_pass - 1) / per_pass, wanted = 32u * static_cast<uint32_t>(multiprocessors()) / tokens;
+    const uint32_t warps = max(1u, min(wanted, passes));
+    const unsigned blocks = static_cast<unsigned>((static_cast<uint64_t>(tokens) * warps + 7) / 8);
+    if (pieces) rotary_pieces_kernel<kBf16, kInterleaved><<<blocks, 256, 0, stream>>>(g, tokens, warps);
+    else rotary_pairs_kernel<kBf16, kInterleaved><<<blocks, 256, 0, stream>>>(g, tokens, warps, copied);
 }
 
 }  // namespace
@@ -132,10 +269,12 @@ extern "C" int krea2_rotary(krea2_stream stream, size_t tokens, const void *q, c
                           static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(head_dim), static_cast<uint32_t>(rotary_dim / 2),
                           q_stride, k_stride, q_out_stride, k_out_stride, magnitude, inverse ? -1.0f : 1.0f};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(tokens);
+    const uint32_t n = static_cast<uint32_t>(tokens);
     const bool interleaved = layout == KREA2_ROTARY_INTERLEAVED;
-    if (kind == KREA2_BF16) interleaved ? rotary_kernel<true, true><<<grid, 256, 0, s>>>(g) : rotary_kernel<true, false><<<grid, 256, 0, s>>>(g);
-    else interleaved ? rotary_kernel<false, true><<<grid, 256, 0, s>>>(g) : rotary_kernel<false, false><<<grid, 256, 0, s>>>(g);
+    const bool aligned = head_dim % 8 == 0 && aligned16(q) && aligned16(q_out) && q_stride % 8 == 0 && q_out_stride % 8 == 0 &&
+                         (kv_heads == 0 || (aligned16(k) && aligned16(k_out) && k_stride % 8 == 0 && k_out_stride % 8 == 0));
+    if (kind == KREA2_BF16) interleaved ? launch_rotary<true, true>(s, n, g, aligned) : launch_rotary<true, false>(s, n, g, aligned);
+    else interleaved ? launch_rotary<false, true>(s, n, g, aligned) : launch_rotary<false, false>(s, n, g, aligned);
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "%s launch failed: %s", name, cudaGetErrorString(status));
     return KREA2_OK;
