@@ -4,9 +4,9 @@
 //   out[b][i][h] = sum_j p_j v[b][j][h'] / sum_j p_j,  p_j = exp(scale q[b][i][h] . k[b][j][h'])
 // over the keys j < kv_lengths[b] whose mask byte is not zero, h' = h / (q_heads / kv_heads); zero where there is none.
 //
-// One pass over the keys with a running maximum and sum.  A CTA owns 128 rows of one key head: the query heads that share
-// it are packed (row r is query r / shares, head r % shares of the key head's), so a single query fills as many rows as
-// heads share its keys.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with f32 accumulators in tensor memory; K and V
+// One pass over the keys with a running maximum and sum.  A CTA owns up to 128 rows of one key head: the query heads that
+// share it are packed (row r is query r / shares, head r % shares of the key head's), so a single query fills as many rows as
+// heads share its keys, and one tile load or store moves the rows of 128 / shares queries.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with f32 accumulators in tensor memory; K and V
 // tiles of 128 keys arrive by TMA as they lie (V is the second product's B operand with its channels innermost, so nothing
 // is transposed), a thread owns one row's softmax and writes P over S in tensor memory.  Two CTAs share an SM: one's
 // softmax, its start and its output run under the other's products.
@@ -23,24 +23,32 @@ namespace {
 __device__ int g_cross_status = 0;  // folded into krea2_device_status by take_cross_status
 constexpr int kCrossTimedOut = 128;
 
+#ifndef KREA2_CROSS_FMA
+#define KREA2_CROSS_FMA 0
+#endif
 constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
 
 struct CrossArgs {
-    const uint16_t *q;
     const int32_t *kv_lengths;
     const uint8_t *key_mask;
     uint16_t *out;
-    uint32_t rows, kv_len, shares, head_dim;  // rows: queries times shares
-    size_t q_batch_stride, q_stride, out_batch_stride, out_stride, mask_stride;
-    uint32_t k_batches, v_batches;  // 1 where every item of the batch shares its keys (values), 0 otherwise
-    float scale_log2;               // softmax scale times log2(e)
+    uint32_t q_len, kv_len, shares, queries, head_dim;  // shares: query heads of a key head; queries of a row tile: 128 / shares
+    size_t out_batch_stride, out_stride, mask_stride;
+    uint32_t q_batches, k_batches, v_batches;  // 1 where every item of the batch shares its queries (keys, values), 0 otherwise
+    float scale_log2;                          // softmax scale times log2(e)
 };
 
 // kD: channels of a head as the tiles hold them, 64 or 128; those past head_dim are zero.
 template <int kD>
 struct Cross {
     static constexpr int kSoftmaxWarps = 4, kLoadWarp = 4, kProductWarp = 5, kValueWarp = 6;
-    static constexpr int kThreads = 7 * 32;
+    static constexpr int kThreads = 8 * 32;  // a warpgroup of softmax, one of the others (and an idle warp)
+    // A row's 128 scores stay in registers: the softmax takes what the other warpgroup does without of the launch's 128.
+    static constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;
+    static_assert(kSoftmaxRegisters + kOtherRegisters <= 2 * 128, "registers of the launch");
+    // Of every eight pairs of weights, those that take the FMA pipes.  The exponential unit does 16 a clock and SM, so that a
+    // tile's 128 x 128 would take it as long as both products together take the tensor cores.
+    static constexpr int kOnFma = KREA2_CROSS_FMA;
     static constexpr int kSubtileBytes = kRows * 128;  // 128 rows of 64 channels: one 128-byte swizzled column block
     static constexpr int kTileBytes = kD / 64 * kSubtileBytes;
     static constexpr int kStages = kD == 64 ? 2 : 1;
@@ -65,6 +73,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^x for both lanes on the FMA pipes, in packed arithmetic, for the share of the weights that the exponential unit is spared:
+// x = n + r with n the nearest integer (adding 1.5 * 2^23 leaves it in the low mantissa bits) and |r| <= 1/2, 2^r by a
+// polynomial of degree 5 (minimax, relative error 2^-22.6), n added into the exponent.  x is clamped at -125, so that the
+// exponent never wraps: such a weight is zero beside the row's largest, and a key that does not count has zeros for values.
+__device__ __forceinline__ float2 exp2_on_fma(float2 x) {
+    const float2 one = make_float2(1.0f, 1.0f), magic = make_float2(12582912.0f, 12582912.0f);
+    x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+    const float2 t = fma_pair(x, one, magic);
+    const float2 n = fma_pair(t, one, make_float2(-12582912.0f, -12582912.0f));
+    const float2 r = fma_pair(n, make_float2(-1.0f, -1.0f), x);
+    float2 p = fma_pair(make_float2(1.3276470126584172e-3f, 1.3276470126584172e-3f), r, make_float2(9.675541892647743e-3f, 9.675541892647743e-3f));
+    p = fma_pair(p, r, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
+    p = fma_pair(p, r, make_float2(2.4022120237350464e-1f, 2.4022120237350464e-1f));
+    p = fma_pair(p, r, make_float2(6.931469440460205e-1f, 6.931469440460205e-1f));
+    p = fma_pair(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 // The largest of three; a NaN among them stays one, so that a row that meets a NaN becomes NaN through its maximum.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -104,14 +130,15 @@ __device__ __forceinline__ void issue_f16_tensor_a(uint32_t tmem, uint32_t a, ui
 
 template <int kD, bool kBf16>
 __global__ void __launch_bounds__(Cross<kD>::kThreads, 2)
-cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const CrossArgs g) {
+cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ CUtensorMap map_out, const CrossArgs g) {
     using T = Cross<kD>;
     extern __shared__ uint8_t shared_raw[];
     uint8_t *q_tile = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(shared_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *k_tiles = q_tile + T::kTileBytes, *v_tiles = k_tiles + T::kStages * T::kTileBytes;
     uint64_t *q_full = reinterpret_cast<uint64_t *>(v_tiles + T::kStages * T::kTileBytes);
     uint64_t *k_full = q_full + 1, *k_empty = k_full + T::kStages, *v_full = k_empty + T::kStages, *v_empty = v_full + T::kStages;
-    uint64_t *v_ready = v_empty + T::kStages, *s_full = v_ready + T::kStages, *p_full = s_full + 1, *o_full = p_full + 1, *words_full = o_full + 1;
+    uint64_t *v_ready = v_empty + T::kStages, *s_full = v_ready + T::kStages, *p_full = s_full + 1, *o_full = p_full + 2, *out_full = o_full + 1, *words_full = out_full + 1;
     uint32_t *words = reinterpret_cast<uint32_t *>(words_full + 2);  // [2][4]: which keys of a tile count, two tiles in turn
     uint32_t *tmem_slot = words + 8;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -121,7 +148,8 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t parts = cluster_size(), rank = cluster_rank();
-    const uint32_t row0 = blockIdx.x / parts * kRows, kv_head = blockIdx.y, batch = blockIdx.z;
+    const uint32_t query0 = blockIdx.x / parts * g.queries, kv_head = blockIdx.y, batch = blockIdx.z;
+    const uint32_t rows = min(g.queries, g.q_len - query0) * g.shares;
     int32_t length = static_cast<int32_t>(g.kv_len);
     if (g.kv_lengths) length = min(max(g.kv_lengths[batch], 0), length);
     const uint32_t keys = static_cast<uint32_t>(length), tiles = (keys + kRows - 1) / kRows;
@@ -131,7 +159,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint32_t issued = 0;  // loader warps: tiles requested
 
     if (threadIdx.x == 0) {
-        barrier_init(q_full, T::kSoftmaxWarps);
+        barrier_init(q_full, 1);
         for (int s = 0; s < T::kStages; s++) {
             barrier_init(k_full + s, 1);
             barrier_init(k_empty + s, 1);
@@ -141,7 +169,9 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         barrier_init(s_full, 1);
         barrier_init(p_full, T::kSoftmaxWarps);
+        barrier_init(p_full + 1, T::kSoftmaxWarps);
         barrier_init(o_full, 1);
+        barrier_init(out_full, T::kSoftmaxWarps);
         barrier_init(words_full, 1);
         barrier_init(words_full + 1, 1);
         *abort_flag = 0;
@@ -158,124 +188,127 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     float reference = -INFINITY, sum = 0.0f;  // a softmax thread's row, in units of log2
     bool alive = true;
 
-    if (warp == T::kLoadWarp) {
-        const bool elected = elect_lane();
-        for (uint32_t i = 0; i < count; i++, issued++) {
-            const uint32_t s = i % T::kStages;
-            if (!barrier_wait_warp(k_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
-            if (elected) {
-                barrier_expect(k_full + s, T::kTileBytes);
+    if (warp >= T::kSoftmaxWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegisters));
+        if (warp == T::kLoadWarp) {
+            const bool elected = elect_lane();
+            if (count && elected) {
+                barrier_expect(q_full, kD / 64 * g.queries * g.shares * 128);
 #pragma unroll
                 for (int sub = 0; sub < kD / 64; sub++)
-                    load_tile_4d(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes, &map_k, k_full + s, sub * 64, static_cast<int>(kv_head),
-                                 static_cast<int>((first + i) * kRows), static_cast<int>(g.k_batches ? 0 : batch));
+                    load_tile_4d(q_tile + sub * T::kSubtileBytes, &map_q, q_full, sub * 64, static_cast<int>(kv_head * g.shares), static_cast<int>(query0),
+                                 static_cast<int>(g.q_batches ? 0 : batch));
             }
             __syncwarp();
-        }
-    } else if (warp == T::kValueWarp) {
-        const bool elected = elect_lane();
-        for (uint32_t i = 0; i < count; i++, issued++) {
-            const uint32_t s = i % T::kStages, key0 = (first + i) * kRows;
-            uint32_t word[4];
+            for (uint32_t i = 0; i < count; i++, issued++) {
+                const uint32_t s = i % T::kStages;
+                if (!barrier_wait_warp(k_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
+                if (elected) {
+                    barrier_expect(k_full + s, T::kTileBytes);
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const uint32_t key = key0 + w * 32 + lane;
-                word[w] = __ballot_sync(0xffffffffu, key < keys && (!g.key_mask || g.key_mask[batch * g.mask_stride + key] != 0));
-            }
-            if (!barrier_wait_warp(v_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
-            if (g.key_mask) {  // the tile that used these words two tiles ago has been through its second product
-                if (lane < 4) words[(i & 1u) * 4 + lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
-                __syncwarp();
-                if (lane == 0) barrier_arrive(words_full + (i & 1u));
-            }
-            uint8_t *tile = v_tiles + s * T::kTileBytes;
-            if (elected) {
-                barrier_expect(v_full + s, T::kTileBytes);
-#pragma unroll
-                for (int sub = 0; sub < kD / 64; sub++)
-                    load_tile_4d(tile + sub * T::kSubtileBytes, &map_v, v_full + s, sub * 64, static_cast<int>(kv_head), static_cast<int>(key0),
-                                 static_cast<int>(g.v_batches ? 0 : batch));
-            }
-            __syncwarp();
-            if (!g.key_mask && key0 + kRows <= keys) continue;
-            // Keys that do not count have the weight zero, but zero times what lies in their values may be NaN: their rows
-            // are cleared before the second product reads the tile.
-            if (!barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort)) break;
-            constexpr uint32_t kPieces = kD / 8;  // 16 bytes each
-#pragma unroll 1
-            for (uint32_t piece = lane; piece < kRows * kPieces; piece += 32) {
-                const uint32_t row = piece / kPieces, at = piece % kPieces;
-                const uint32_t bits = row < 32 ? word[0] : row < 64 ? word[1] : row < 96 ? word[2] : word[3];
-                if (!((bits >> (row & 31u)) & 1u))
-                    *reinterpret_cast<uint4 *>(tile + (at >> 3) * T::kSubtileBytes + row * 128 + (at & 7u) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) barrier_arrive(v_ready + s);
-        }
-    } else if (warp == T::kProductWarp) {
-        const bool elected = elect_lane();
-        constexpr uint32_t scores_idesc = attention_descriptor<kBf16>(kRows, false), values_idesc = attention_descriptor<kBf16>(kD, true);
-        if (count) alive = barrier_wait_warp(q_full, 0, abort);
-        // The pipe runs one thread's products in issue order and a commit covers all that was issued before it: the scores of
-        // a tile overwrite the weights of the one before only after the second product has read them, and the softmax that
-        // sees new scores may rescale O.
-        auto scores = [&](uint32_t i) {
-            const uint32_t s = i % T::kStages;
-            if (!barrier_wait_warp(k_full + s, (i / T::kStages) & 1u, abort)) return false;
-            tensor_fence_after();
-            if (elected) {
-#pragma unroll
-                for (int sub = 0; sub < kD / 64; sub++) {
-                    const uint64_t a = operand_descriptor(smem_address(q_tile + sub * T::kSubtileBytes));
-                    const uint64_t b = operand_descriptor(smem_address(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) issue_f16(tmem, a + 2 * k, b + 2 * k, scores_idesc, sub != 0 || k != 0);
+                    for (int sub = 0; sub < kD / 64; sub++)
+                        load_tile_4d(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes, &map_k, k_full + s, sub * 64, static_cast<int>(kv_head),
+                                     static_cast<int>((first + i) * kRows), static_cast<int>(g.k_batches ? 0 : batch));
                 }
-                tensor_commit(s_full);
-                tensor_commit(k_empty + s);
+                __syncwarp();
             }
-            __syncwarp();
-            return true;
-        };
-        if (count && alive) alive = scores(0);
-        for (uint32_t i = 0; alive && i < count; i++) {
-            const uint32_t s = i % T::kStages;
-            const bool cleared = g.key_mask || (first + i + 1) * kRows > keys;
-            alive = cleared ? barrier_wait_warp(v_ready + s, g.key_mask ? (i / T::kStages) & 1u : 0u, abort)
-                            : barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort);
-            alive = alive && barrier_wait_warp(p_full, i & 1u, abort);
-            if (!alive) break;
-            tensor_fence_after();
-            if (elected) {
+        } else if (warp == T::kValueWarp) {
+            const bool elected = elect_lane();
+            for (uint32_t i = 0; i < count; i++, issued++) {
+                const uint32_t s = i % T::kStages, key0 = (first + i) * kRows;
+                uint32_t word[4];
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t key = key0 + w * 32 + lane;
+                    word[w] = __ballot_sync(0xffffffffu, key < keys && (!g.key_mask || g.key_mask[batch * g.mask_stride + key] != 0));
+                }
+                if (!barrier_wait_warp(v_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
+                if (g.key_mask) {  // the tile that used these words two tiles ago has been through its second product
+                    if (lane < 4) words[(i & 1u) * 4 + lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(words_full + (i & 1u));
+                }
+                uint8_t *tile = v_tiles + s * T::kTileBytes;
+                if (elected) {
+                    barrier_expect(v_full + s, T::kTileBytes);
+#pragma unroll
+                    for (int sub = 0; sub < kD / 64; sub++)
+                        load_tile_4d(tile + sub * T::kSubtileBytes, &map_v, v_full + s, sub * 64, static_cast<int>(kv_head), static_cast<int>(key0),
+                                     static_cast<int>(g.v_batches ? 0 : batch));
+                }
+                __syncwarp();
+                if (!g.key_mask && key0 + kRows <= keys) continue;
+                // Keys that do not count have the weight zero, but zero times what lies in their values may be NaN: their rows
+                // are cleared before the second product reads the tile.
+                if (!barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort)) break;
+                constexpr uint32_t kPieces = kD / 8;  // 16 bytes each
+#pragma unroll 1
+                for (uint32_t piece = lane; piece < kRows * kPieces; piece += 32) {
+                    const uint32_t row = piece / kPieces, at = piece % kPieces;
+                    const uint32_t bits = row < 32 ? word[0] : row < 64 ? word[1] : row < 96 ? word[2] : word[3];
+                    if (!((bits >> (row & 31u)) & 1u))
+                        *reinterpret_cast<uint4 *>(tile + (at >> 3) * T::kSubtileBytes + row * 128 + (at & 7u) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(v_ready + s);
+            }
+        } else if (warp == T::kProductWarp) {
+            const bool elected = elect_lane();
+            constexpr uint32_t scores_idesc = attention_descriptor<kBf16>(kRows, false), values_idesc = attention_descriptor<kBf16>(kD, true);
+            if (count) alive = barrier_wait_warp(q_full, 0, abort);
+            // The pipe runs one thread's products in issue order and a commit covers all that was issued before it: the scores of
+            // a tile overwrite the weights of the one before only after the second product has read them, and the softmax that
+            // sees new scores may rescale O.
+            auto scores = [&](uint32_t i) {
+                const uint32_t s = i % T::kStages;
+                if (!barrier_wait_warp(k_full + s, (i / T::kStages) & 1u, abort)) return false;
+                tensor_fence_after();
+                if (elected) {
+#pragma unroll
+                    for (int sub = 0; sub < kD / 64; sub++) {
+                        const uint64_t a = operand_descriptor(smem_address(q_tile + sub * T::kSubtileBytes));
+                        const uint64_t b = operand_descriptor(smem_address(k_tiles + s * T::kTileBytes + sub * T::kSubtileBytes));
+#pragma unroll
+                        for (int k = 0; k < 4; k++) issue_f16(tmem, a + 2 * k, b + 2 * k, scores_idesc, sub != 0 || k != 0);
+                    }
+                    tensor_commit(s_full);
+                    tensor_commit(k_empty + s);
+                }
+                __syncwarp();
+                return true;
+            };
+            if (count && alive) alive = scores(0);
+            for (uint32_t i = 0; alive && i < count; i++) {
+                const uint32_t s = i % T::kStages;
+                const bool cleared = g.key_mask || (first + i + 1) * kRows > keys;
+                alive = cleared ? barrier_wait_warp(v_ready + s, g.key_mask ? (i / T::kStages) & 1u : 0u, abort)
+                                : barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort);
+                // The weights arrive in halves: the first half's products run under the softmax of the second.
                 const uint64_t v = value_descriptor(smem_address(v_tiles + s * T::kTileBytes), T::kSubtileBytes);
 #pragma unroll
-                for (int k = 0; k < kRows / 16; k++) issue_f16_tensor_a(tmem + kRows, tmem + 8 * k, v + 128 * k, values_idesc, i != 0 || k != 0);
-                tensor_commit(v_empty + s);
-                if (i + 1 == count) tensor_commit(o_full);
+                for (int half = 0; half < 2; half++) {
+                    alive = alive && barrier_wait_warp(p_full + half, i & 1u, abort);
+                    if (!alive) break;
+                    tensor_fence_after();
+                    if (elected) {
+#pragma unroll
+                        for (int k = 4 * half; k < 4 * half + 4; k++)
+                            issue_f16_tensor_a(tmem + kRows, tmem + 8 * k, v + 128 * k, values_idesc, i != 0 || k != 0);
+                        if (half == 1) {
+                            tensor_commit(v_empty + s);
+                            if (i + 1 == count) tensor_commit(o_full);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!alive) break;
+                if (i + 1 < count) alive = scores(i + 1);
             }
-            __syncwarp();
-            if (i + 1 < count) alive = scores(i + 1);
         }
     } else {
         // ---- softmax: thread = row
-        if (count) {
-            // The warp's 32 rows of Q, 16 bytes a piece, into the swizzled layout; what is past the rows or the head is zero.
-            constexpr uint32_t kPieces = kD / 8;
-#pragma unroll 4
-            for (uint32_t piece = lane; piece < 32 * kPieces; piece += 32) {
-                const uint32_t local = warp * 32 + piece / kPieces, at = piece % kPieces, row = row0 + local;
-                const bool inside = row < g.rows && at * 8 < g.head_dim;
-                const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
-                const uint16_t *from = g.q + (inside ? batch * g.q_batch_stride + query * g.q_stride + static_cast<size_t>(head) * g.head_dim + at * 8 : 0);
-                const uint32_t to = smem_address(q_tile + (at >> 3) * T::kSubtileBytes + local * 128 + (((at & 7u) ^ (local & 7u)) * 16));
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(inside ? 16u : 0u) : "memory");
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) barrier_arrive(q_full);
-        }
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftmaxRegisters));
         const uint32_t lane_bits = static_cast<uint32_t>(warp * 32) << 16;
         const uint32_t s_at = tmem + lane_bits, o_at = tmem + kRows + lane_bits;
         for (uint32_t i = 0; i < count; i++) {
@@ -297,35 +330,33 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             if (!(alive = barrier_wait_warp(s_full, i & 1u, abort))) break;
             tensor_fence_after();
-            // The 128 scores pass through registers twice, 64 at a time: for the maximum and for the weights.
-            auto load_half = [&](int half, float (&v)[64]) {
-                tensor_load_32(s_at + half * 64, v);
-                tensor_load_32(s_at + half * 64 + 32, v + 32);
-                tensor_loads_done();
-                if (!all) {
+            float v[kRows];
 #pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        if (!((word[2 * half + (k >> 5)] >> (k & 31)) & 1u)) v[k] = -INFINITY;
-                }
-            };
-            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int c = 0; c < 4; c++) tensor_load_32(s_at + c * 32, v + c * 32);
+            tensor_loads_done();
+            if (!all) {
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float v[64];
-                load_half(half, v);
-#pragma unroll
-                for (int k = 0; k < 64; k += 8)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) part[t] = max3_nan(part[t], v[k + t], v[k + 4 + t]);
+                for (int k = 0; k < kRows; k++)
+                    if (!((word[k >> 5] >> (k & 31)) & 1u)) v[k] = -INFINITY;
             }
-            const float top = max_nan(max3_nan(part[0], part[1], part[2]), part[3]) * g.scale_log2;
+            float part[8];
+#pragma unroll
+            for (int t = 0; t < 8; t++) part[t] = max3_nan(v[t], v[8 + t], v[16 + t]);
+#pragma unroll
+            for (int k = 24; k < kRows - 8; k += 16)
+#pragma unroll
+                for (int t = 0; t < 8; t++) part[t] = max3_nan(part[t], v[k + t], v[k + 8 + t]);
+#pragma unroll
+            for (int t = 0; t < 8; t++) part[t] = max_nan(part[t], v[kRows - 8 + t]);
+            const float top = max3_nan(max3_nan(part[0], part[1], part[2]), max3_nan(part[3], part[4], part[5]), max_nan(part[6], part[7])) * g.scale_log2;
             // The exponents' reference moves only when the maximum has grown by more than 2^8 (a weight of 256 is exact
-            // enough in either type, and neither O nor the sum changes its ratio); a NaN moves it for good.
+            // enough in either type, and neither O nor the sum changes its ratio); NaN and infinity make the row NaN for good.
             float alpha = 1.0f;
             const bool move = !(top <= reference + 8.0f);
             if (move) {
-                alpha = exp2_approx(reference - top);
-                reference = top;
+                const float next = top < INFINITY ? top : NAN;
+                alpha = exp2_approx(reference - next);
+                reference = next;
                 sum *= alpha;
             }
             if (i > 0 && __any_sync(0xffffffffu, move)) {
@@ -341,34 +372,37 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 tensor_stores_done();
             }
             const float shift = reference == -INFINITY ? 0.0f : -reference;  // nothing counted yet: the weights are zero, not NaN
-            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float2 total[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) total[t] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                float v[64];
-                load_half(half, v);
                 uint32_t packed[32];
 #pragma unroll
-                for (int k = 0; k < 64; k += 2) {
-                    const float2 x = fma_pair(make_float2(v[k], v[k + 1]), make_float2(g.scale_log2, g.scale_log2), make_float2(shift, shift));
-                    const float p0 = exp2_approx(x.x), p1 = exp2_approx(x.y);
-                    total[(k >> 1) & 3] += p0 + p1;
-                    packed[k / 2] = pack_pair<kBf16>(p0, p1);
+                for (int k = 0; k < 32; k++) {
+                    const float2 x = fma_pair(make_float2(v[64 * half + 2 * k], v[64 * half + 2 * k + 1]), make_float2(g.scale_log2, g.scale_log2),
+                                              make_float2(shift, shift));
+                    const float2 p = k % 8 < 8 - T::kOnFma ? make_float2(exp2_approx(x.x), exp2_approx(x.y)) : exp2_on_fma(x);
+                    total[k & 3] = add_pair(total[k & 3], p);
+                    packed[k] = pack_pair<kBf16>(p.x, p.y);
                 }
                 tensor_store_32(s_at + half * 32, packed);
+                tensor_stores_done();
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(p_full + half);
             }
-            sum += (total[0] + total[1]) + (total[2] + total[3]);
-            tensor_stores_done();
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(p_full);
+            total[0] = add_pair(add_pair(total[0], total[1]), add_pair(total[2], total[3]));
+            sum += total[0].x + total[0].y;
         }
         alive = alive && (count == 0 || barrier_wait_warp(o_full, 0, abort));
         tensor_fence_after();
         if (alive && parts == 1) {
-            // Through the warp's own rows of the Q tile (no product reads it any more), so that rows leave in pieces of 128 bytes.
+            // Through the Q tile, which no product reads any more: one tile store moves all rows (and leaves out the queries
+            // past the last).
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
             const uint32_t local = warp * 32 + lane;
-#pragma unroll 1
+#pragma unroll
             for (int c = 0; c < kD; c += 32) {
                 float o[32];
                 if (count) {
@@ -384,17 +418,19 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     *reinterpret_cast<uint4 *>(q_tile + (at >> 3) * T::kSubtileBytes + local * 128 + (((at & 7u) ^ (local & 7u)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            constexpr uint32_t kPieces = kD / 8;
-#pragma unroll 4
-            for (uint32_t piece = lane; piece < 32 * kPieces; piece += 32) {
-                const uint32_t mine = warp * 32 + piece / kPieces, at = piece % kPieces, row = row0 + mine;
-                if (row >= g.rows || at * 8 >= g.head_dim) continue;
-                const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
-                *reinterpret_cast<uint4 *>(g.out + batch * g.out_batch_stride + query * g.out_stride + static_cast<size_t>(head) * g.head_dim + at * 8) =
-                    *reinterpret_cast<const uint4 *>(q_tile + (at >> 3) * T::kSubtileBytes + mine * 128 + (((at & 7u) ^ (mine & 7u)) * 16));
+            if (lane == 0) barrier_arrive(out_full);
+            if (threadIdx.x == 0 && barrier_wait(out_full, 0, abort)) {
+#pragma unroll
+                for (int sub = 0; sub < kD / 64; sub++)
+                    if (sub * 64 < g.head_dim)
+                        store_tile_4d(q_tile + sub * T::kSubtileBytes, &map_out, sub * 64, static_cast<int>(kv_head * g.shares), static_cast<int>(query0),
+                                      static_cast<int>(batch));
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the tile has to outlive the reading
             }
-        } else if (alive && row0 + warp * 32 < g.rows) {
+        } else if (alive && static_cast<uint32_t>(warp * 32) < rows) {
             // A share of the keys: the row's reference, sum and unscaled output for the others to read.
             const uint32_t local = warp * 32 + lane;
             stats[2 * local] = reference;
@@ -420,6 +456,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (*abort_flag && (warp == T::kLoadWarp || warp == T::kValueWarp) && lane == 0) {
         uint64_t *full = warp == T::kLoadWarp ? k_full : v_full;
         const uint64_t start = clock_ns();
+        if (warp == T::kLoadWarp && count) barrier_drain(q_full, 0, start);
         for (uint32_t i = issued > T::kStages ? issued - T::kStages : 0u; i < issued; i++) barrier_drain(full + i % T::kStages, (i / T::kStages) & 1u, start);
     }
     if (warp == T::kProductWarp) {
@@ -428,9 +465,9 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
     if (parts == 1) return;
     cluster_barrier();  // every share of this row tile is in shared memory
-    const uint32_t rows_here = min(static_cast<uint32_t>(kRows), g.rows - row0), pieces = g.head_dim / 4;
-    for (uint32_t item = threadIdx.x * parts + rank; item < rows_here * pieces; item += T::kThreads * parts) {
-        const uint32_t local = item / pieces, at = item % pieces, row = row0 + local;
+    const uint32_t pieces = g.head_dim / 4;
+    for (uint32_t item = threadIdx.x * parts + rank; item < rows * pieces; item += T::kThreads * parts) {
+        const uint32_t local = item / pieces, at = item % pieces;
         float references[8], top = -INFINITY, total = 0.0f;
         float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f), share[8];
         float sums[8];
@@ -453,7 +490,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             value.x += weight * share[r].x, value.y += weight * share[r].y, value.z += weight * share[r].z, value.w += weight * share[r].w;
         }
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-        const uint32_t query = row / g.shares, head = kv_head * g.shares + row % g.shares;
+        const uint32_t query = query0 + local / g.shares, head = kv_head * g.shares + local % g.shares;
         *reinterpret_cast<uint2 *>(g.out + batch * g.out_batch_stride + query * g.out_stride + static_cast<size_t>(head) * g.head_dim + at * 4) =
             make_uint2(pack_pair<kBf16>(value.x * inverse, value.y * inverse), pack_pair<kBf16>(value.z * inverse, value.w * inverse));
     }
@@ -461,16 +498,21 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 }
 
 // ---------------------------------------------------------------- host side
-// Keys or values [batch][kv_len][heads][head_dim] as boxes of 64 channels of one head x 128 rows.
-int states_map(CUtensorMap *map, bool bf16, const void *base, size_t head_dim, size_t heads, size_t rows, size_t batch, size_t stride, size_t batch_stride) {
+// [batch][rows][heads][head_dim] as boxes of 64 channels of `box_heads` heads and `box_rows` rows.
+int states_map(CUtensorMap *map, bool bf16, const void *base, size_t head_dim, size_t heads, size_t rows, size_t batch, size_t stride, size_t batch_stride,
+               uint32_t box_heads, uint32_t box_rows) {
     const cuuint64_t dims[4] = {head_dim, heads, rows, batch};
     const cuuint64_t strides[3] = {head_dim * 2, stride * 2, batch > 1 ? batch_stride * 2 : stride * 2};
-    const cuuint32_t box[4] = {64, 1, kRows, 1};
+    const cuuint32_t box[4] = {64, box_heads, box_rows, 1};
     return make_tensor_map(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box);
 }
 
+struct CrossMaps {
+    CUtensorMap q, k, v, out;
+};
+
 template <int kD, bool kBf16>
-int launch_cross(cudaStream_t stream, const CUtensorMap &map_k, const CUtensorMap &map_v, size_t batch, size_t kv_heads, const CrossArgs &g) {
+int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_t kv_heads, const CrossArgs &g) {
     using T = Cross<kD>;
     static Prepared prepared;
     static std::atomic<int> known[64][9];  // clusters of so many CTAs that a device holds at once
@@ -486,7 +528,7 @@ int launch_cross(cudaStream_t stream, const CUtensorMap &map_k, const CUtensorMa
     attribute.val.clusterDim.x = attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    const uint32_t row_tiles = (g.rows + kRows - 1) / kRows, key_tiles = (g.kv_len + kRows - 1) / kRows;
+    const uint32_t row_tiles = (g.q_len + g.queries - 1) / g.queries, key_tiles = (g.kv_len + kRows - 1) / kRows;
     const size_t tiles = row_tiles * batch * kv_heads;
     // The keys are split as far as all clusters stay resident; each share has a tile of keys at least.
     uint32_t parts = 1;
@@ -504,7 +546,7 @@ int launch_cross(cudaStream_t stream, const CUtensorMap &map_k, const CUtensorMa
     }
     attribute.val.clusterDim.x = parts;
     config.gridDim = dim3(row_tiles * parts, static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
-    const cudaError_t status = cudaLaunchKernelEx(&config, cross_attention_kernel<kD, kBf16>, map_k, map_v, g);
+    const cudaError_t status = cudaLaunchKernelEx(&config, cross_attention_kernel<kD, kBf16>, maps.q, maps.k, maps.v, maps.out, g);
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "cross_attention launch failed: %s", cudaGetErrorString(status));
     return KREA2_OK;
 }
@@ -551,19 +593,21 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
     KREA2_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "%s: buffers must be 16-byte aligned", name);
     KREA2_REQUIRE(reinterpret_cast<uintptr_t>(kv_lengths) % 4 == 0, "%s: kv_lengths must be 4-byte aligned", name);
     const size_t shares = q_heads / kv_heads;
-    KREA2_REQUIRE(q_len * shares <= 0x7fffff00 / 8, "%s: %zu queries of %zu heads to a key head exceed the grid", name, q_len, shares);
-    const bool bf16 = kind == KREA2_BF16, k_shared = batch > 1 && k_batch_stride == 0, v_shared = batch > 1 && v_batch_stride == 0;
-    const CrossArgs g = {static_cast<const uint16_t *>(q), kv_lengths, static_cast<const uint8_t *>(key_mask), static_cast<uint16_t *>(out),
-                         static_cast<uint32_t>(q_len * shares), static_cast<uint32_t>(kv_len), static_cast<uint32_t>(shares), static_cast<uint32_t>(head_dim),
-                         q_batch_stride, q_stride, out_batch_stride, out_stride, mask_stride, k_shared ? 1u : 0u, v_shared ? 1u : 0u,
-                         scale * 1.44269504088896340736f};
-    CUtensorMap map_k = {}, map_v = {};  // without keys no load is issued
+    KREA2_REQUIRE(shares <= kRows, "%s: %zu query heads share a key head, %d are served", name, shares, kRows);
+    const uint32_t queries = static_cast<uint32_t>(kRows / shares), h = static_cast<uint32_t>(shares);
+    const bool bf16 = kind == KREA2_BF16, q_shared = batch > 1 && q_batch_stride == 0, k_shared = batch > 1 && k_batch_stride == 0,
+               v_shared = batch > 1 && v_batch_stride == 0;
+    const CrossArgs g = {kv_lengths, static_cast<const uint8_t *>(key_mask), static_cast<uint16_t *>(out), static_cast<uint32_t>(q_len),
+                         static_cast<uint32_t>(kv_len), h, queries, static_cast<uint32_t>(head_dim), out_batch_stride, out_stride, mask_stride,
+                         q_shared ? 1u : 0u, k_shared ? 1u : 0u, v_shared ? 1u : 0u, scale * 1.44269504088896340736f};
+    CrossMaps maps = {};  // without keys none is loaded
+    if (int status = states_map(&maps.q, bf16, q, head_dim, q_heads, q_len, q_shared ? 1 : batch, q_stride, q_batch_stride, h, queries)) return status;
+    if (int status = states_map(&maps.out, bf16, out, head_dim, q_heads, q_len, batch, out_stride, out_batch_stride, h, queries)) return status;
     if (kv_len != 0) {
-        if (int status = states_map(&map_k, bf16, k, head_dim, kv_heads, kv_len, k_shared ? 1 : batch, k_stride, k_batch_stride)) return status;
-        if (int status = states_map(&map_v, bf16, v, head_dim, kv_heads, kv_len, v_shared ? 1 : batch, v_stride, v_batch_stride)) return status;
+        if (int status = states_map(&maps.k, bf16, k, head_dim, kv_heads, kv_len, k_shared ? 1 : batch, k_stride, k_batch_stride, 1, kRows)) return status;
+        if (int status = states_map(&maps.v, bf16, v, head_dim, kv_heads, kv_len, v_shared ? 1 : batch, v_stride, v_batch_stride, 1, kRows)) return status;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (head_dim <= 64)
-        return bf16 ? launch_cross<64, true>(s, map_k, map_v, batch, kv_heads, g) : launch_cross<64, false>(s, map_k, map_v, batch, kv_heads, g);
-    return bf16 ? launch_cross<128, true>(s, map_k, map_v, batch, kv_heads, g) : launch_cross<128, false>(s, map_k, map_v, batch, kv_heads, g);
+    if (head_dim <= 64) return bf16 ? launch_cross<64, true>(s, maps, batch, kv_heads, g) : launch_cross<64, false>(s, maps, batch, kv_heads, g);
+    return bf16 ? launch_cross<128, true>(s, maps, batch, kv_heads, g) : launch_cross<128, false>(s, maps, batch, kv_heads, g);
 }

@@ -163,6 +163,12 @@ __device__ __forceinline__ void load_tile_4d(void *dst, const CUtensorMap *map, 
         ::"r"(smem_address(dst)), "l"(map), "r"(smem_address(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
         : "memory");
 }
+// Shared memory to a tile; what lies outside the tensor is left out.  The caller commits and waits for the group.
+__device__ __forceinline__ void store_tile_4d(const void *src, const CUtensorMap *map, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_address(src)), "r"(c0), "r"(c1),
+                 "r"(c2), "r"(c3)
+                 : "memory");
+}
 
 // ---------------------------------------------------------------- tensor memory
 template <int kCtas>
@@ -246,6 +252,13 @@ __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
         " fma.rn.f32x2 s, p, q, r;\n mov.b64 {%0, %1}, s;\n }"
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n add.rn.f32x2 r, p, q;\n mov.b64 {%0, %1}, r;\n }"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
 
