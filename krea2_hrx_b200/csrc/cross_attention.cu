@@ -23,9 +23,6 @@ namespace {
 __device__ int g_cross_status = 0;  // folded into krea2_device_status by take_cross_status
 constexpr int kCrossTimedOut = 128;
 
-#ifndef KREA2_CROSS_FMA
-#define KREA2_CROSS_FMA 0
-#endif
 constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
 
 struct CrossArgs {
@@ -41,14 +38,11 @@ struct CrossArgs {
 // kD: channels of a head as the tiles hold them, 64 or 128; those past head_dim are zero.
 template <int kD>
 struct Cross {
-    static constexpr int kSoftmaxWarps = 4, kLoadWarp = 4, kProductWarp = 5, kValueWarp = 6;
-    static constexpr int kThreads = 8 * 32;  // a warpgroup of softmax, one of the others (and an idle warp)
+    static constexpr int kSoftmaxWarps = 4, kLoadWarp = 4, kProductWarp = 5, kValueWarp = 6, kMaskWarp = 7;
+    static constexpr int kThreads = 8 * 32;  // a warpgroup of softmax, one of the others
     // A row's 128 scores stay in registers: the softmax takes what the other warpgroup does without of the launch's 128.
     static constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;
     static_assert(kSoftmaxRegisters + kOtherRegisters <= 2 * 128, "registers of the launch");
-    // Of every eight pairs of weights, those that take the FMA pipes.  The exponential unit does 16 a clock and SM, so that a
-    // tile's 128 x 128 would take it as long as both products together take the tensor cores.
-    static constexpr int kOnFma = KREA2_CROSS_FMA;
     static constexpr int kSubtileBytes = kRows * 128;  // 128 rows of 64 channels: one 128-byte swizzled column block
     static constexpr int kTileBytes = kD / 64 * kSubtileBytes;
     static constexpr int kStages = kD == 64 ? 2 : 1;
@@ -73,24 +67,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// 2^x for both lanes on the FMA pipes, in packed arithmetic, for the share of the weights that the exponential unit is spared:
-// x = n + r with n the nearest integer (adding 1.5 * 2^23 leaves it in the low mantissa bits) and |r| <= 1/2, 2^r by a
-// polynomial of degree 5 (minimax, relative error 2^-22.6), n added into the exponent.  x is clamped at -125, so that the
-// exponent never wraps: such a weight is zero beside the row's largest, and a key that does not count has zeros for values.
-__device__ __forceinline__ float2 exp2_on_fma(float2 x) {
-    const float2 one = make_float2(1.0f, 1.0f), magic = make_float2(12582912.0f, 12582912.0f);
-    x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
-    const float2 t = fma_pair(x, one, magic);
-    const float2 n = fma_pair(t, one, make_float2(-12582912.0f, -12582912.0f));
-    const float2 r = fma_pair(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = fma_pair(make_float2(1.3276470126584172e-3f, 1.3276470126584172e-3f), r, make_float2(9.675541892647743e-3f, 9.675541892647743e-3f));
-    p = fma_pair(p, r, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
-    p = fma_pair(p, r, make_float2(2.4022120237350464e-1f, 2.4022120237350464e-1f));
-    p = fma_pair(p, r, make_float2(6.931469440460205e-1f, 6.931469440460205e-1f));
-    p = fma_pair(p, r, make_float2(1.0000001192092896f, 1.0000001192092896f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 // The largest of three; a NaN among them stays one, so that a row that meets a NaN becomes NaN through its maximum.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -128,6 +104,12 @@ __device__ __forceinline__ void issue_f16_tensor_a(uint32_t tmem, uint32_t a, ui
                  : "memory");
 }
 
+// Which keys of a tile count where the first `left` of them do.
+__device__ __forceinline__ void tail_words(uint32_t left, uint32_t (&word)[4]) {
+#pragma unroll
+    for (uint32_t w = 0; w < 4; w++) word[w] = left >= 32 * w + 32 ? 0xffffffffu : left <= 32 * w ? 0u : (1u << (left - 32 * w)) - 1u;
+}
+
 template <int kD, bool kBf16>
 __global__ void __launch_bounds__(Cross<kD>::kThreads, 2)
 cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -139,8 +121,8 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     uint64_t *q_full = reinterpret_cast<uint64_t *>(v_tiles + T::kStages * T::kTileBytes);
     uint64_t *k_full = q_full + 1, *k_empty = k_full + T::kStages, *v_full = k_empty + T::kStages, *v_empty = v_full + T::kStages;
     uint64_t *v_ready = v_empty + T::kStages, *s_full = v_ready + T::kStages, *p_full = s_full + 1, *o_full = p_full + 2, *out_full = o_full + 1, *words_full = out_full + 1;
-    uint32_t *words = reinterpret_cast<uint32_t *>(words_full + 2);  // [2][4]: which keys of a tile count, two tiles in turn
-    uint32_t *tmem_slot = words + 8;
+    uint32_t *words = reinterpret_cast<uint32_t *>(words_full + 4);  // [4][4]: which keys of a tile count, four tiles in turn
+    uint32_t *tmem_slot = words + 16;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *stats = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(q_full) + T::kBarrierBytes);  // [128][2]: reference and sum of a row
     float *partial = reinterpret_cast<float *>(k_tiles);                                              // [128][kD], once the products are done
@@ -172,8 +154,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         barrier_init(p_full + 1, T::kSoftmaxWarps);
         barrier_init(o_full, 1);
         barrier_init(out_full, T::kSoftmaxWarps);
-        barrier_init(words_full, 1);
-        barrier_init(words_full + 1, 1);
+        for (int s = 0; s < 4; s++) barrier_init(words_full + s, 1);
         *abort_flag = 0;
         barrier_init_done();
     }
@@ -190,6 +171,26 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 
     if (warp >= T::kSoftmaxWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegisters));
+        // Keys that do not count have the weight zero, but zero times what lies in their values may be NaN: a warp clears their
+        // rows once the tile is there and before the second product reads it.
+        auto clear = [&](uint32_t i, const uint32_t (&word)[4]) {
+            const uint32_t s = i % T::kStages;
+            if (!barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort)) return false;
+            uint8_t *tile = v_tiles + s * T::kTileBytes;
+            constexpr uint32_t kPieces = kD / 8, kAtOnce = 32 / kPieces;  // of 16 bytes in a row, rows
+            const uint32_t at = lane % kPieces, base = (at >> 3) * T::kSubtileBytes + (at & 7u) * 16;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (word[w] == 0xffffffffu) continue;
+#pragma unroll 4
+                for (uint32_t bit = lane / kPieces; bit < 32; bit += kAtOnce)
+                    if (!((word[w] >> bit) & 1u)) *reinterpret_cast<uint4 *>(tile + base + (w * 32 + bit) * 128) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) barrier_arrive(v_ready + s);
+            return true;
+        };
         if (warp == T::kLoadWarp) {
             const bool elected = elect_lane();
             if (count && elected) {
@@ -215,43 +216,51 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         } else if (warp == T::kValueWarp) {
             const bool elected = elect_lane();
             for (uint32_t i = 0; i < count; i++, issued++) {
-                const uint32_t s = i % T::kStages, key0 = (first + i) * kRows;
-                uint32_t word[4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const uint32_t key = key0 + w * 32 + lane;
-                    word[w] = __ballot_sync(0xffffffffu, key < keys && (!g.key_mask || g.key_mask[batch * g.mask_stride + key] != 0));
-                }
+                const uint32_t s = i % T::kStages;
                 if (!barrier_wait_warp(v_empty + s, ((i / T::kStages) & 1u) ^ 1u, abort)) break;
-                if (g.key_mask) {  // the tile that used these words two tiles ago has been through its second product
-                    if (lane < 4) words[(i & 1u) * 4 + lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
-                    __syncwarp();
-                    if (lane == 0) barrier_arrive(words_full + (i & 1u));
-                }
-                uint8_t *tile = v_tiles + s * T::kTileBytes;
                 if (elected) {
                     barrier_expect(v_full + s, T::kTileBytes);
 #pragma unroll
                     for (int sub = 0; sub < kD / 64; sub++)
-                        load_tile_4d(tile + sub * T::kSubtileBytes, &map_v, v_full + s, sub * 64, static_cast<int>(kv_head), static_cast<int>(key0),
-                                     static_cast<int>(g.v_batches ? 0 : batch));
+                        load_tile_4d(v_tiles + s * T::kTileBytes + sub * T::kSubtileBytes, &map_v, v_full + s, sub * 64, static_cast<int>(kv_head),
+                                     static_cast<int>((first + i) * kRows), static_cast<int>(g.v_batches ? 0 : batch));
                 }
                 __syncwarp();
-                if (!g.key_mask && key0 + kRows <= keys) continue;
-                // Keys that do not count have the weight zero, but zero times what lies in their values may be NaN: their rows
-                // are cleared before the second product reads the tile.
-                if (!barrier_wait_warp(v_full + s, (i / T::kStages) & 1u, abort)) break;
-                constexpr uint32_t kPieces = kD / 8;  // 16 bytes each
-#pragma unroll 1
-                for (uint32_t piece = lane; piece < kRows * kPieces; piece += 32) {
-                    const uint32_t row = piece / kPieces, at = piece % kPieces;
-                    const uint32_t bits = row < 32 ? word[0] : row < 64 ? word[1] : row < 96 ? word[2] : word[3];
-                    if (!((bits >> (row & 31u)) & 1u))
-                        *reinterpret_cast<uint4 *>(tile + (at >> 3) * T::kSubtileBytes + row * 128 + (at & 7u) * 16) = make_uint4(0, 0, 0, 0);
+                if (!g.key_mask && (first + i + 1) * kRows > keys) {
+                    uint32_t word[4];
+                    tail_words(keys - (first + i) * kRows, word);
+                    if (!clear(i, word)) break;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+        } else if (warp == T::kMaskWarp && g.key_mask) {
+            // Which keys of a tile count goes to the softmax two tiles ahead, and their values are cleared as they land.  (Every
+            // tile of a masked launch waits for this warp, so that it meets each phase of the barriers.)
+            auto words_of = [&](uint32_t i, uint32_t (&word)[4]) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t key = (first + i) * kRows + w * 32 + lane;
+                    word[w] = __ballot_sync(0xffffffffu, i < count && key < keys && g.key_mask[batch * g.mask_stride + key] != 0);
+                }
+            };
+            auto publish = [&](uint32_t i, const uint32_t (&word)[4]) {
+                if (i >= count) return;
+                if (lane < 4) words[(i & 3u) * 4 + lane] = lane == 0 ? word[0] : lane == 1 ? word[1] : lane == 2 ? word[2] : word[3];
                 __syncwarp();
-                if (lane == 0) barrier_arrive(v_ready + s);
+                if (lane == 0) barrier_arrive(words_full + (i & 3u));
+            };
+            uint32_t word[4], next[4], after[4];
+            words_of(0, word);
+            words_of(1, next);
+            publish(0, word);
+            publish(1, next);
+            for (uint32_t i = 0; i < count; i++) {
+                words_of(i + 2, after);
+                if (!clear(i, word)) break;
+                // The tile that used these words four tiles ago has been through its second product: this tile's values came
+                // in its place or a later one's.
+                publish(i + 2, after);
+#pragma unroll
+                for (int w = 0; w < 4; w++) word[w] = next[w], next[w] = after[w];
             }
         } else if (warp == T::kProductWarp) {
             const bool elected = elect_lane();
@@ -316,17 +325,13 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             const uint32_t key0 = (first + i) * kRows;
             bool all = true;
             if (g.key_mask) {
-                if (!(alive = barrier_wait_warp(words_full + (i & 1u), (i >> 1) & 1u, abort))) break;
+                if (!(alive = barrier_wait_warp(words_full + (i & 3u), (i >> 2) & 1u, abort))) break;
 #pragma unroll
-                for (int w = 0; w < 4; w++) word[w] = words[(i & 1u) * 4 + w];
+                for (int w = 0; w < 4; w++) word[w] = words[(i & 3u) * 4 + w];
                 all = (word[0] & word[1] & word[2] & word[3]) == 0xffffffffu;
             } else if (key0 + kRows > keys) {
                 all = false;
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int32_t here = static_cast<int32_t>(keys - key0) - 32 * w;
-                    word[w] = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1u;
-                }
+                tail_words(keys - key0, word);
             }
             if (!(alive = barrier_wait_warp(s_full, i & 1u, abort))) break;
             tensor_fence_after();
@@ -382,7 +387,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int k = 0; k < 32; k++) {
                     const float2 x = fma_pair(make_float2(v[64 * half + 2 * k], v[64 * half + 2 * k + 1]), make_float2(g.scale_log2, g.scale_log2),
                                               make_float2(shift, shift));
-                    const float2 p = k % 8 < 8 - T::kOnFma ? make_float2(exp2_approx(x.x), exp2_approx(x.y)) : exp2_on_fma(x);
+                    const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
                     total[k & 3] = add_pair(total[k & 3], p);
                     packed[k] = pack_pair<kBf16>(p.x, p.y);
                 }
@@ -530,9 +535,11 @@ int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_
     config.numAttrs = 1;
     const uint32_t row_tiles = (g.q_len + g.queries - 1) / g.queries, key_tiles = (g.kv_len + kRows - 1) / kRows;
     const size_t tiles = row_tiles * batch * kv_heads;
-    // The keys are split as far as all clusters stay resident; each share has a tile of keys at least.
+    // The split of the keys that takes least by the measured parts: a tile of keys 1.9 us, a CTA's start and end 4 us, the
+    // addition of the shares 3 us; CTAs beyond those that are resident at once run in further rounds.
     uint32_t parts = 1;
-    for (uint32_t more = 2; more <= 8 && more <= key_tiles; more++) {
+    float least = INFINITY;
+    for (uint32_t more = 1; more <= 8 && more <= (key_tiles ? key_tiles : 1u); more++) {
         int clusters = known[device][more].load(std::memory_order_relaxed);
         if (clusters == 0) {
             config.gridDim = dim3(more, 1, 1);
@@ -541,8 +548,9 @@ int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_
             if (clusters < 1) clusters = 1;
             known[device][more].store(clusters, std::memory_order_relaxed);
         }
-        if (tiles > static_cast<size_t>(clusters)) break;
-        parts = more;
+        const float rounds = static_cast<float>((tiles + clusters - 1) / clusters);
+        const float time = rounds * (1.9f * static_cast<float>((key_tiles + more - 1) / more) + (more > 1 ? 7.0f : 4.0f));
+        if (time < least) least = time, parts = more;
     }
     attribute.val.clusterDim.x = parts;
     config.gridDim = dim3(row_tiles * parts, static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));

@@ -272,81 +272,103 @@ def _kind(name, t: torch.Tensor) -> int:
     return kind
 
 
-def _check_rows(name, what, t, shape, dtype, device, lead=1) -> None:
-    """A tensor of that shape and type on that device whose dimensions after the first `lead` lie in one piece."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise InvalidArgument(f"{name}: {what} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    if t.device != device or not t.is_cuda:
+def _dims(name, t: torch.Tensor, rank: int):
+    if t.dim() != rank:
+        raise InvalidArgument(f"{name}: a tensor of {rank} dimensions is needed, got {tuple(t.shape)}")
+    return t.shape
+
+
+def _rows(name, what, t, shape, dtype, device, inner, lead=1) -> int:
+    """Elements from one row of `t` to the next, where it has that shape and type, lies on that device and its dimensions
+    after the first `lead` in one piece of `inner` elements.  A lone row's stride carries no meaning: it counts as `inner`."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise InvalidArgument(f"{name}: {what} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
         raise InvalidArgument(f"{name}: {what} is on {t.device}: buffers must share one CUDA device")
-    if not t.is_contiguous():
-        inner, strides = 1, t.stride()
-        for i in range(len(shape) - 1, lead - 1, -1):
-            if shape[i] != 1 and strides[i] != inner:
-                raise InvalidArgument(f"{name}: the rows of {what} must be contiguous")
-            inner *= shape[i]
+    if t.is_contiguous():
+        return inner
+    size, strides = 1, t.stride()
+    for i in range(len(shape) - 1, lead - 1, -1):
+        if shape[i] != 1 and strides[i] != size:
+            raise InvalidArgument(f"{name}: the rows of {what} must be contiguous")
+        size *= shape[i]
+    return strides[lead - 1] if shape[lead - 1] > 1 else inner
 
 
-def _row_stride(t: torch.Tensor, inner: int) -> int:
-    """Elements from one row to the next; a lone row's stride carries no meaning."""
-    return t.stride(0) if t.shape[0] > 1 else inner
+def _pitch(t: torch.Tensor, stride: int) -> int:
+    """The row pitch of codes: that of a lone row, whatever it says, is taken as the next multiple of 16."""
+    return stride if t.shape[0] > 1 else _padded(stride)
 
 
 def _padded(stride: int) -> int:
     return -(-stride // 16) * 16
 
 
+# The current stream of a device as a pointer; torch.cuda.current_stream() takes 3 us of a small call's 12.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _run_on(name, device: torch.device, stream, fn, *args) -> None:
+    if device.type != "cuda":
+        raise InvalidArgument(f"{name}: buffers must live on a CUDA device")
+    index = device.index
     if stream is not None and stream.device != device:
         raise InvalidArgument(f"{name}: the stream belongs to {stream.device}, the buffers to {device}")
-    if device.index == torch.cuda.current_device():
-        check(fn((stream or torch.cuda.current_stream()).cuda_stream, *args))
+    pointer = stream.cuda_stream if stream is not None else _raw_stream(index)
+    if index == torch.cuda.current_device():
+        status = fn(pointer, *args)
     else:
-        with torch.cuda.device(device):
-            check(fn((stream or torch.cuda.current_stream()).cuda_stream, *args))
+        with torch.cuda.device(index):
+            status = fn(pointer, *args)
+    if status:
+        check(status)
 
 
 def prepare_norm_fp8(x, weight, q, q_scale, residual=None, sum_out=None, eps=1e-5, weight_offset=0.0, stream=None):
     """RMS norm of x [tokens][width] (after x + residual, which `sum_out` receives, if there is one) times
     (weight_offset + weight), as e4m3 codes q with q_scale f32 [tokens][ceil(width/128)]."""
-    name, device, (tokens, width) = "prepare_norm_fp8", x.device, x.shape
-    kind = _kind(name, x)
-    _check_rows(name, "x", x, (tokens, width), x.dtype, device)
-    _check_rows(name, "q", q, (tokens, width), torch.float8_e4m3fn, device)
-    _check_rows(name, "q_scale", q_scale, (tokens, _groups(width)), torch.float32, device)
-    for what, t in (("residual", residual), ("sum_out", sum_out)):
-        if t is not None:
-            _check_rows(name, what, t, (tokens, width), x.dtype, device)
-    if weight is not None and (weight.dtype != torch.float32 or weight.numel() != width or weight.device != device):
-        raise InvalidArgument(f"{name}: weight must be float32 [{width}] on {device}")
-    _run_on(name, device, stream, lib().krea2_prepare_norm_fp8, tokens, x.data_ptr(), residual.data_ptr() if residual is not None else None,
-            _ptr(weight) if weight is not None else None, sum_out.data_ptr() if sum_out is not None else None, q.data_ptr(), _ptr(q_scale),
-            width, _row_stride(x, width), _row_stride(residual, width) if residual is not None else 0,
-            _row_stride(sum_out, width) if sum_out is not None else 0, _row_stride(q, _padded(width)), eps, weight_offset, kind)
+    name, device, shape, dtype = "prepare_norm_fp8", x.device, x.shape, x.dtype
+    kind, (tokens, width) = _kind(name, x), _dims(name, x, 2)
+    x_stride = _rows(name, "x", x, shape, dtype, device, width)
+    q_stride = _pitch(q, _rows(name, "q", q, shape, torch.float8_e4m3fn, device, width))
+    _rows(name, "q_scale", q_scale, (tokens, -(-width // GROUP)), torch.float32, device, width)
+    residual_ptr = weight_ptr = sum_ptr = None
+    residual_stride = sum_stride = 0
+    if residual is not None:
+        residual_stride, residual_ptr = _rows(name, "residual", residual, shape, dtype, device, width), residual.data_ptr()
+    if sum_out is not None:
+        sum_stride, sum_ptr = _rows(name, "sum_out", sum_out, shape, dtype, device, width), sum_out.data_ptr()
+    if weight is not None:
+        if weight.dtype is not torch.float32 or weight.numel() != width or weight.device != device:
+            raise InvalidArgument(f"{name}: weight must be float32 [{width}] on {device}")
+        weight_ptr = _ptr(weight)
+    _run_on(name, device, stream, lib().krea2_prepare_norm_fp8, tokens, x.data_ptr(), residual_ptr, weight_ptr, sum_ptr, q.data_ptr(), _ptr(q_scale),
+            width, x_stride, residual_stride, sum_stride, q_stride, eps, weight_offset, kind)
 
 
 def prepare_plain_fp8(x, q, q_scale, stream=None):
     """e4m3 codes of x [tokens][width] with one scale per 128 channels (prepare_norm_fp8 without the norm)."""
-    name, device, (tokens, width) = "prepare_plain_fp8", x.device, x.shape
-    kind = _kind(name, x)
-    _check_rows(name, "x", x, (tokens, width), x.dtype, device)
-    _check_rows(name, "q", q, (tokens, width), torch.float8_e4m3fn, device)
-    _check_rows(name, "q_scale", q_scale, (tokens, _groups(width)), torch.float32, device)
-    _run_on(name, device, stream, lib().krea2_prepare_plain_fp8, tokens, x.data_ptr(), q.data_ptr(), _ptr(q_scale), width,
-            _row_stride(x, width), _row_stride(q, _padded(width)), kind)
+    name, device, shape = "prepare_plain_fp8", x.device, x.shape
+    kind, (tokens, width) = _kind(name, x), _dims(name, x, 2)
+    x_stride = _rows(name, "x", x, shape, x.dtype, device, width)
+    q_stride = _pitch(q, _rows(name, "q", q, shape, torch.float8_e4m3fn, device, width))
+    _rows(name, "q_scale", q_scale, (tokens, -(-width // GROUP)), torch.float32, device, width)
+    _run_on(name, device, stream, lib().krea2_prepare_plain_fp8, tokens, x.data_ptr(), q.data_ptr(), _ptr(q_scale), width, x_stride, q_stride, kind)
 
 
 def gemm_fp8_128(a, a_scale, w, w_scale, c, stream=None):
     """c [m][n] (f16 or bf16) = a [m][k] times w [n][k] transposed, e4m3 codes under a_scale f32 [m][ceil(k/128)] and
     w_scale f32 [ceil(n/128)][ceil(k/128)]."""
-    name, device, (m, k), n = "gemm_fp8_128", a.device, a.shape, w.shape[0]
-    kind = _kind(name, c)
-    _check_rows(name, "a", a, (m, k), torch.float8_e4m3fn, device)
-    _check_rows(name, "w", w, (n, k), torch.float8_e4m3fn, device)
-    _check_rows(name, "a_scale", a_scale, (m, _groups(k)), torch.float32, device)
-    _check_rows(name, "w_scale", w_scale, (_groups(n), _groups(k)), torch.float32, device)
-    _check_rows(name, "c", c, (m, n), c.dtype, device)
-    _run_on(name, device, stream, lib().krea2_gemm_fp8_128, m, a.data_ptr(), w.data_ptr(), _ptr(w_scale), _ptr(a_scale), c.data_ptr(), k,
-            _row_stride(a, _padded(k)), _row_stride(w, _padded(k)), n, _row_stride(c, n), kind)
+    name, device = "gemm_fp8_128", a.device
+    kind, (m, k), (n, _) = _kind(name, c), _dims(name, a, 2), _dims(name, w, 2)
+    groups = -(-k // GROUP)
+    a_stride = _pitch(a, _rows(name, "a", a, a.shape, torch.float8_e4m3fn, device, k))
+    w_stride = _pitch(w, _rows(name, "w", w, (n, k), torch.float8_e4m3fn, device, k))
+    _rows(name, "a_scale", a_scale, (m, groups), torch.float32, device, groups)
+    _rows(name, "w_scale", w_scale, (-(-n // GROUP), groups), torch.float32, device, groups)
+    c_stride = _rows(name, "c", c, (m, n), c.dtype, device, n)
+    _run_on(name, device, stream, lib().krea2_gemm_fp8_128, m, a.data_ptr(), w.data_ptr(), _ptr(w_scale), _ptr(a_scale), c.data_ptr(), k, a_stride,
+            w_stride, n, c_stride, kind)
 
 
 class QuantizedFp8:
@@ -415,54 +437,59 @@ def rotary(q, k, q_out, k_out, frequencies, positions=None, magnitude=1.0, layou
     """Turns q [tokens][q_heads][head_dim] and k [tokens][kv_heads][head_dim] (or None) by positions * frequencies into
     q_out and k_out, which may be q and k; the first 2 * len(frequencies) channels of a head take part.  inverse=True is
     the gradient's way back."""
-    name, device, (tokens, q_heads, head_dim) = "rotary", q.device, q.shape
-    kind, kv_heads = _kind(name, q), 0
-    for what, t in (("q", q), ("q_out", q_out)):
-        _check_rows(name, what, t, (tokens, q_heads, head_dim), q.dtype, device)
+    name, device, shape, dtype = "rotary", q.device, q.shape, q.dtype
+    kind, (tokens, q_heads, head_dim) = _kind(name, q), _dims(name, q, 3)
+    row = q_heads * head_dim
+    q_stride, q_out_stride = _rows(name, "q", q, shape, dtype, device, row), _rows(name, "q_out", q_out, shape, dtype, device, row)
+    kv_heads = k_stride = k_out_stride = 0
+    k_ptr = k_out_ptr = positions_ptr = None
     if (k is None) != (k_out is None):
         raise InvalidArgument(f"{name}: k and k_out go together")
     if k is not None:
-        kv_heads = k.shape[1]
-        for what, t in (("k", k), ("k_out", k_out)):
-            _check_rows(name, what, t, (tokens, kv_heads, head_dim), q.dtype, device)
+        kv_heads = _dims(name, k, 3)[1]
+        shape, row = (tokens, kv_heads, head_dim), kv_heads * head_dim
+        k_stride, k_out_stride = _rows(name, "k", k, shape, dtype, device, row), _rows(name, "k_out", k_out, shape, dtype, device, row)
+        k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
     if layout not in ROTARY_LAYOUTS:
         raise InvalidArgument(f"{name}: layout is one of {', '.join(ROTARY_LAYOUTS)}")
-    if frequencies.dtype != torch.float64 or frequencies.device != device:
+    if frequencies.dtype is not torch.float64 or frequencies.device != device:
         raise InvalidArgument(f"{name}: frequencies must be float64 on {device}")
-    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != tokens or positions.device != device):
-        raise InvalidArgument(f"{name}: positions must be int32 [{tokens}] on {device}")
-    q_row, k_row = q_heads * head_dim, kv_heads * head_dim
-    _run_on(name, device, stream, lib().krea2_rotary, tokens, q.data_ptr(), k.data_ptr() if kv_heads else None,
-            _ptr(positions) if positions is not None else None, _ptr(frequencies), q_out.data_ptr(), k_out.data_ptr() if kv_heads else None,
-            q_heads, kv_heads, head_dim, 2 * frequencies.numel(), _row_stride(q, q_row), _row_stride(k, k_row) if kv_heads else 0,
-            _row_stride(q_out, q_row), _row_stride(k_out, k_row) if kv_heads else 0, magnitude, ROTARY_LAYOUTS[layout], int(bool(inverse)), kind)
+    if positions is not None:
+        if positions.dtype is not torch.int32 or positions.numel() != tokens or positions.device != device:
+            raise InvalidArgument(f"{name}: positions must be int32 [{tokens}] on {device}")
+        positions_ptr = _ptr(positions)
+    _run_on(name, device, stream, lib().krea2_rotary, tokens, q.data_ptr(), k_ptr, positions_ptr, _ptr(frequencies), q_out.data_ptr(), k_out_ptr,
+            q_heads, kv_heads, head_dim, 2 * frequencies.numel(), q_stride, k_stride, q_out_stride, k_out_stride, magnitude, ROTARY_LAYOUTS[layout],
+            1 if inverse else 0, kind)
 
 
 def cross_attention(q, k, v, out, kv_lengths=None, key_mask=None, scale=None, stream=None):
     """Attention of q [batch][q_len][q_heads][head_dim] to an encoder's k, v [batch][kv_len][kv_heads][head_dim], written
     to `out` (shaped like q).  kv_lengths int32 [batch] and key_mask bool or uint8 [batch][kv_len] say which keys count
     (both: those that both name); a query without one gets zeros.  scale defaults to head_dim ** -0.5."""
-    name, device, (batch, q_len, q_heads, head_dim) = "cross_attention", q.device, q.shape
-    kind, kv_len, kv_heads = _kind(name, q), k.shape[1], k.shape[2]
-    for what, t in (("q", q), ("out", out)):
-        _check_rows(name, what, t, (batch, q_len, q_heads, head_dim), q.dtype, device, 2)
-    for what, t in (("k", k), ("v", v)):
-        _check_rows(name, what, t, (batch, kv_len, kv_heads, head_dim), q.dtype, device, 2)
-    if kv_lengths is not None and (kv_lengths.dtype != torch.int32 or kv_lengths.numel() != batch or kv_lengths.device != device):
-        raise InvalidArgument(f"{name}: kv_lengths must be int32 [{batch}] on {device}")
+    name, device, shape, dtype = "cross_attention", q.device, q.shape, q.dtype
+    kind, (batch, q_len, q_heads, head_dim), (_, kv_len, kv_heads, _) = _kind(name, q), _dims(name, q, 4), _dims(name, k, 4)
+
+    def strides(what, t, shape, row):
+        """(batch stride, row stride)"""
+        stride = _rows(name, what, t, shape, dtype, device, row, 2)
+        if batch == 1 or t.is_contiguous():
+            return shape[1] * stride, stride
+        return t.stride()[0], stride
+
+    q_row, kv_row, kv_shape = q_heads * head_dim, kv_heads * head_dim, (batch, kv_len, kv_heads, head_dim)
+    q_strides, out_strides = strides("q", q, shape, q_row), strides("out", out, shape, q_row)
+    k_strides, v_strides = strides("k", k, kv_shape, kv_row), strides("v", v, kv_shape, kv_row)
+    lengths_ptr = mask_ptr = None
     mask_stride = 0
+    if kv_lengths is not None:
+        if kv_lengths.dtype is not torch.int32 or kv_lengths.numel() != batch or kv_lengths.device != device:
+            raise InvalidArgument(f"{name}: kv_lengths must be int32 [{batch}] on {device}")
+        lengths_ptr = _ptr(kv_lengths)
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8):
             raise InvalidArgument(f"{name}: key_mask must be bool or uint8")
-        _check_rows(name, "key_mask", key_mask, (batch, kv_len), key_mask.dtype, device)
-        mask_stride = _row_stride(key_mask, kv_len)
-    q_row, k_row = q_heads * head_dim, kv_heads * head_dim
-
-    def strides(t, row):
-        rows = t.stride(1) if t.shape[1] > 1 else row
-        return (t.stride(0) if batch > 1 else t.shape[1] * rows), rows
-
-    _run_on(name, device, stream, lib().krea2_cross_attention, batch, q_len, kv_len, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            _ptr(kv_lengths) if kv_lengths is not None else None, key_mask.data_ptr() if key_mask is not None else None, out.data_ptr(),
-            q_heads, kv_heads, head_dim, *strides(q, q_row), *strides(k, k_row), *strides(v, k_row), *strides(out, q_row), mask_stride,
+        mask_stride, mask_ptr = _rows(name, "key_mask", key_mask, (batch, kv_len), key_mask.dtype, device, kv_len), key_mask.data_ptr()
+    _run_on(name, device, stream, lib().krea2_cross_attention, batch, q_len, kv_len, q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths_ptr, mask_ptr,
+            out.data_ptr(), q_heads, kv_heads, head_dim, *q_strides, *k_strides, *v_strides, *out_strides, mask_stride,
             head_dim ** -0.5 if scale is None else scale, kind)
