@@ -128,7 +128,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     float *partial = reinterpret_cast<float *>(k_tiles);                                              // [128][kD], once the products are done
     const Abort abort = {abort_flag, &g_cross_status, kCrossTimedOut};
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const uint32_t parts = cluster_size(), rank = cluster_rank();
     const uint32_t query0 = blockIdx.x / parts * g.queries, kv_head = blockIdx.y, batch = blockIdx.z;
     const uint32_t rows = min(g.queries, g.q_len - query0) * g.shares;
@@ -165,7 +165,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     float reference = -INFINITY, sum = 0.0f;  // a softmax thread's row, in units of log2
     bool alive = true;
 

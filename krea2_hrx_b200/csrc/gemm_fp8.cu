@@ -185,7 +185,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const T::Scales scales = {reinterpret_cast<float *>(staging + T::kWarps * T::kStagingBytes), scale_full, scale_empty};
     const Abort abort = {abort_flag, &g_product_status, kProductTimedOut};
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -227,7 +227,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     tensor_fence_before();
     cluster_barrier();
     tensor_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     if (warp >= T::kWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegisters));
         if (warp == T::kWarps && lane == 0) {
@@ -256,16 +256,16 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             constexpr uint32_t idesc = product_descriptor(2 * T::kRows, T::kColumns / 2);
             uint32_t stage = 0, phase = 0, count = 0;
             bool alive = true;
+            bool loaded = false, free0 = false, free1 = false;  // what the next block's barriers said while this one's products ran
             for (uint32_t tile = pair; alive && tile < tiles; tile += pairs) {
                 for (uint32_t b = 0; b < g.blocks; b++, count++) {
-                    const uint32_t s = count & 1u;
+                    const uint32_t s = count & 1u, parity = ((count >> 1) & 1u) ^ 1u;
                     const uint32_t at = smem_address(shared + stage * T::kStageBytes);
                     const uint64_t a = operand_descriptor(at);
+                    if (!(alive = barrier_wait_warp(full + stage, phase, abort, loaded))) break;
 #pragma unroll
                     for (uint32_t half = 0; half < 2; half++) {
-                        if (!(alive = alive && barrier_wait_warp(sum_empty + 2 * half + s, ((count >> 1) & 1u) ^ 1u, abort) &&
-                                      (half != 0 || barrier_wait_warp(full + stage, phase, abort))))
-                            break;
+                        if (!(alive = barrier_wait_warp(sum_empty + 2 * half + s, parity, abort, half == 0 ? free0 : free1))) break;
                         tensor_fence_after();
                         // each CTA holds 128 of the tile's rows of w: its 64 of this half lie at 64 * half
                         const uint64_t w = operand_descriptor(at + T::kOperandBytes + half * (T::kOperandBytes / 2));
@@ -280,6 +280,10 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     }
                     if (!alive) break;
                     if (++stage == T::kStages) stage = 0, phase ^= 1u;
+                    const uint32_t next = (count + 1) & 1u, next_parity = (((count + 1) >> 1) & 1u) ^ 1u;
+                    loaded = barrier_peek(full + stage, phase);
+                    free0 = barrier_peek(sum_empty + next, next_parity);
+                    free1 = barrier_peek(sum_empty + 2 + next, next_parity);
                 }
             }
         }
@@ -308,6 +312,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             float2 out[T::kWarpColumns / 2];
 #pragma unroll
             for (int i = 0; i < T::kWarpColumns / 2; i++) out[i] = make_float2(0.0f, 0.0f);
+            bool ready = false;
             for (uint32_t b = 0; b < g.blocks; b++, count++) {
                 const uint32_t s = count & 1u;
                 if ((b & 3u) == 0u && !(alive = barrier_wait_warp(scale_full + run % T::Scales::kSlots, T::Scales::parity(run), abort))) break;
@@ -319,7 +324,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (lane == 0) barrier_arrive(scale_empty + run % T::Scales::kSlots);
                     run++;
                 }
-                if (!(alive = barrier_wait_warp(sum_full + 2 * half + s, (count >> 1) & 1u, abort))) break;
+                if (!(alive = barrier_wait_warp(sum_full + 2 * half + s, (count >> 1) & 1u, abort, ready))) break;
                 tensor_fence_after();
                 const uint32_t from = tmem + s * T::kColumns + half * T::kWarpColumns + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
@@ -331,6 +336,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         tensor_fence_before();
                         __syncwarp();
                         if (lane == 0) barrier_arrive_at(release[s]);
+                        ready = barrier_peek(sum_full + 2 * half + (s ^ 1u), ((count + 1) >> 1) & 1u);
                     }
 #pragma unroll
                     for (int i = 0; i < 8; i++) out[c * 8 + i] = fma_pair(make_float2(sums[2 * i], sums[2 * i + 1]), scale, out[c * 8 + i]);
@@ -418,7 +424,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     float *partial = reinterpret_cast<float *>(shared);                                     // [kTokens][kPitch], once the stages are done with
     const Abort abort = {abort_flag, &g_product_status, kProductTimedOut};
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x, shares = gridDim.x;  // a cluster spans x: the split of the blocks
     const uint32_t n0 = blockIdx.y * T::kRows, m0 = blockIdx.z * kTokens;
     const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(g.blocks) * rank / shares);
@@ -448,7 +454,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
     if (warp == T::kWarps) {
         if (lane == 0) {
@@ -465,9 +471,10 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         {
             const bool elected = elect_lane();
             constexpr uint32_t idesc = product_descriptor(T::kRows, kTokens);
-            for (uint32_t b = first, count = 0; b < last; b++, count++) {
-                const uint32_t s = count % T::kSums, stage = count % T::kStages;
-                if (!barrier_wait_warp(sum_empty + s, ((count / T::kSums) & 1u) ^ 1u, abort) || !barrier_wait_warp(full + stage, (count / T::kStages) & 1u, abort)) break;
+            bool loaded = false, free = false;  // what the next block's barriers said while this one's products ran
+            uint32_t s = 0, stage = 0, sum_phase = 1, load_phase = 0;
+            for (uint32_t b = first; b < last; b++) {
+                if (!barrier_wait_warp(full + stage, load_phase, abort, loaded) || !barrier_wait_warp(sum_empty + s, sum_phase, abort, free)) break;
                 tensor_fence_after();
                 const uint32_t at = smem_address(shared + stage * T::kStageBytes);
                 const uint64_t w = operand_descriptor(at), a = operand_descriptor(at + T::kRows * kBlock);
@@ -478,6 +485,10 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     tensor_commit(sum_full + s);
                 }
                 __syncwarp();
+                if (++stage == T::kStages) stage = 0, load_phase ^= 1u;
+                if (++s == T::kSums) s = 0, sum_phase ^= 1u;
+                loaded = barrier_peek(full + stage, load_phase);
+                free = barrier_peek(sum_empty + s, sum_phase);
             }
         }
     } else if (warp >= T::kWarps + 2) {
@@ -495,11 +506,12 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int i = 0; i < T::kColumns / 8; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) out[i][r] = make_float2(0.0f, 0.0f);
-        uint32_t run = 0;
+        uint32_t run = 0, s = 0, sum_phase = 0;
+        bool ready = false;
         for (uint32_t b = first, count = 0; b < last; b++, count++) {
-            const uint32_t s = count % T::kSums, k = count & 3u;
+            const uint32_t k = count & 3u;
             if (k == 0u && !barrier_wait_warp(scale_full + run % T::Scales::kSlots, T::Scales::parity(run), abort)) break;
-            if (!barrier_wait_warp(sum_full + s, (count / T::kSums) & 1u, abort)) break;
+            if (!barrier_wait_warp(sum_full + s, sum_phase, abort, ready)) break;
             tensor_fence_after();
             const uint32_t from = tmem + s * kTokens + group * T::kColumns + (static_cast<uint32_t>(quarter * 32) << 16);
             const float *mine = scales.slot(run) + k * kTokens + group * T::kColumns + 2 * (lane & 3);
@@ -516,6 +528,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     tensor_fence_before();
                     __syncwarp();
                     if (lane == 0) barrier_arrive(sum_empty + s);
+                    if (++s == T::kSums) s = 0, sum_phase ^= 1u;
+                    ready = barrier_peek(sum_full + s, sum_phase);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++)

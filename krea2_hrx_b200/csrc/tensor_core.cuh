@@ -46,6 +46,20 @@ __device__ __forceinline__ bool barrier_test(uint64_t *bar, uint32_t parity) {
         : "memory");
     return done != 0;
 }
+// The same without the time that a try_wait may spend before it answers no.
+__device__ __forceinline__ bool barrier_peek(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_address(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
 // How a CTA's roles give up together: the CTA's flag, the device's status word and the bit to raise there.
 struct Abort {
     volatile int *flag;
@@ -75,8 +89,11 @@ __device__ __forceinline__ bool barrier_wait(uint64_t *bar, uint32_t parity, con
         if (patience.over(abort)) return false;
     return true;
 }
-// The same for a converged warp, whose lanes leave together: 60 clocks where the phase is complete, 130 lane by lane.
-__device__ __forceinline__ bool barrier_wait_warp(uint64_t *bar, uint32_t parity, const Abort &abort) {
+// The same for a converged warp, whose lanes leave together.  `ready` is what an earlier barrier_peek() of this phase said: a
+// loop that peeks at its next barriers before the work at hand has their answers when it comes back (a wait that is met takes
+// some 130 clocks, as long as the tensor cores take for a quarter of a block).
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t *bar, uint32_t parity, const Abort &abort, bool ready = false) {
+    if (__all_sync(0xffffffffu, ready)) return true;
     Patience patience;
     while (!__all_sync(0xffffffffu, barrier_test(bar, parity)))
         if (__any_sync(0xffffffffu, patience.over(abort))) return false;
@@ -88,6 +105,10 @@ __device__ __forceinline__ void barrier_drain(uint64_t *bar, uint32_t parity, ui
     while (!barrier_test(bar, parity))
         if (clock_ns() - start > kTensorWaitLimitNs) return;
 }
+
+// A value that all lanes hold alike, taken from lane 0: what depends on it is compiled as uniform, and the products' operands
+// need not be moved to uniform registers one by one.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // True in one lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_lane() {
