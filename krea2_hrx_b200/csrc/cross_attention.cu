@@ -338,7 +338,8 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             float v[kRows];
 #pragma unroll
             for (int c = 0; c < 4; c++) tensor_load_32(s_at + c * 32, v + c * 32);
-            tensor_loads_done();
+#pragma unroll
+            for (int c = 0; c < 4; c++) tensor_loads_done_32(v + c * 32);
             if (!all) {
 #pragma unroll
                 for (int k = 0; k < kRows; k++)
@@ -369,7 +370,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 for (int c = 0; c < kD; c += 32) {
                     float o[32];
                     tensor_load_32(o_at + c, o);
-                    tensor_loads_done();
+                    tensor_loads_done_32(o);
 #pragma unroll
                     for (int k = 0; k < 32; k++) o[k] *= alpha;
                     tensor_store_32(o_at + c, reinterpret_cast<const uint32_t *>(o));
@@ -412,7 +413,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 float o[32];
                 if (count) {
                     tensor_load_32(o_at + c, o);
-                    tensor_loads_done();
+                    tensor_loads_done_32(o);
                 }
 #pragma unroll
                 for (int k = 0; k < 32; k += 8) {
@@ -445,7 +446,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 float o[32];
                 if (count) {
                     tensor_load_32(o_at + c, o);
-                    tensor_loads_done();
+                    tensor_loads_done_32(o);
                 }
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)

@@ -331,7 +331,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 for (int c = 0; c < T::kWarpColumns / 16; c++) {
                     float sums[16];
                     tensor_load_16(from + c * 16, sums);
-                    tensor_loads_done();
+                    tensor_loads_done_16(sums);
                     if (c == T::kWarpColumns / 16 - 1) {  // everything has been read: the accumulator may be overwritten
                         tensor_fence_before();
                         __syncwarp();
@@ -517,13 +517,13 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             const float *mine = scales.slot(run) + k * kTokens + group * T::kColumns + 2 * (lane & 3);
 #pragma unroll
             for (int c = 0; c < T::kColumns; c += 16) {
-                float sums[2][8];
-                tensor_load_fragment(from + c, sums[0]);
-                tensor_load_fragment(from + c + (16u << 16), sums[1]);
+                float sums[16];  // rows lane / 4 + 0 and 8, then + 16 and 24
+                tensor_load_fragment(from + c, sums);
+                tensor_load_fragment(from + c + (16u << 16), sums + 8);
                 float2 scale[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) scale[j] = *reinterpret_cast<const float2 *>(mine + c + 8 * j);
-                tensor_loads_done();
+                tensor_loads_done_16(sums);
                 if (c + 16 == T::kColumns) {
                     tensor_fence_before();
                     __syncwarp();
@@ -535,7 +535,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 for (int j = 0; j < 2; j++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float *sum = sums[r >> 1] + 4 * j + 2 * (r & 1);
+                        const float *sum = sums + 8 * (r >> 1) + 4 * j + 2 * (r & 1);
                         out[c / 8 + j][r] = fma_pair(make_float2(sum[0], sum[1]), scale[j], out[c / 8 + j][r]);
                     }
             }

@@ -211,7 +211,6 @@ __device__ __forceinline__ void tensor_free(uint32_t address, uint32_t columns) 
 }
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tensor_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tensor_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Once the products issued so far have completed, arrives on the barrier (of both CTAs of a pair).
 __device__ __forceinline__ void tensor_commit(uint64_t *bar) {
@@ -223,7 +222,7 @@ __device__ __forceinline__ void tensor_commit_pair(uint64_t *bar) {
                  : "memory");
 }
 // 32 lanes x 16 or 32 consecutive 32-bit columns: thread i of the warp receives (or stores) lane base + i.  The loads
-// return before the values are there: tensor_loads_done() completes all that were issued.
+// return before the values are there: a tensor_loads_done completes all that were issued.
 __device__ __forceinline__ void tensor_load_16(uint32_t address, float *r) {
     uint32_t *u = reinterpret_cast<uint32_t *>(r);
     asm volatile(
@@ -243,6 +242,23 @@ __device__ __forceinline__ void tensor_load_32(uint32_t address, float *r) {
           "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]),
           "=r"(u[31])
         : "r"(address));
+}
+// Waits for all loads that were issued; tied to the values, so that nothing that uses them can be moved in front of it.
+__device__ __forceinline__ void tensor_loads_done_16(float *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tensor_loads_done_32(float *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]),
+                   "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]),
+                   "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+                 :
+                 : "memory");
 }
 // 16 lanes x 16 columns in the fragment order: r[4 j + 0], r[4 j + 1] are columns 8 j + 2 (lane % 4) and the one after it of
 // lane base + lane / 4, r[4 j + 2], r[4 j + 3] the same columns eight lanes below.  A thread meets a quarter of the columns.
