@@ -302,7 +302,7 @@ enum { KREA2_F16 = 0, KREA2_BF16 = 1 };
 /* Codes q e4m3 [tokens][out_stride] with one scale per 128 channels, q_scale f32 [tokens][ceil(width/128)]:
  * scale = max(max|y| / 448, 2^-126), code = e4m3(y * (1/scale)) to nearest even.  y is the row x itself, or
  * x / sqrt(mean(x^2) + eps) * (weight_offset + weight[i]) where x has first become kind(x + residual) if there is a
- * residual (`sum`, if not NULL, receives it: it may be the buffer of x or of residual).  weight f32 [width] or NULL for
+ * residual (`sum`, if not NULL, receives it: it may be x or residual, with that stride).  weight f32 [width] or NULL for
  * zeros; weight_offset 1 suits weights stored minus one, as this library's checkpoints hold them, 0 plain ones.  A NaN
  * stays a NaN code in its place; an infinity makes its group (after a norm: its place) NaN.  width 1..32768, out_stride
  * a multiple of 16. */
@@ -342,8 +342,9 @@ int krea2_rotary_frequencies(size_t rotary_dim, double base, int scaling, double
  * kv_heads).  A key counts if j < kv_lengths[b] (int32 [batch], clamped to 0..kv_len; NULL: kv_len) and key_mask
  * (bytes [batch][mask_stride]; NULL: all) is not zero there; whatever lies in keys and values that do not count, NaN
  * included, changes nothing, and a row without a counting key is written as zeros.  q, out [batch][q_len][q_heads *
- * head_dim], k, v [batch][kv_len][kv_heads * head_dim] at 16-byte aligned rows (strides multiples of 8); head_dim a
- * multiple of 8 up to 128, at most 128 query heads to a key head; kv_len may be 0; scale > 0. */
+ * head_dim], k, v [batch][kv_len][kv_heads * head_dim] at 16-byte aligned rows (strides multiples of 8); a batch stride
+ * of 0 (of q, k, v or the mask) shares one item with the whole batch.  head_dim a multiple of 8 up to 128, at most 128
+ * query heads to a key head; kv_len may be 0; scale > 0. */
 int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q_len, size_t kv_len, const void *q, const void *k,
                           const void *v, const int32_t *kv_lengths, const void *key_mask, void *out, size_t q_heads,
                           size_t kv_heads, size_t head_dim, size_t q_batch_stride, size_t q_stride,

@@ -594,8 +594,10 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
                   "%s: a key row holds %zu values, the strides are %zu and %zu", name, kv_heads * head_dim, k_stride, v_stride);
     KREA2_REQUIRE((q_batch_stride | q_stride | k_batch_stride | k_stride | v_batch_stride | v_stride | out_batch_stride | out_stride) % 8 == 0,
                   "%s: strides must be multiples of 8 elements", name);
-    KREA2_REQUIRE(batch == 1 || out_batch_stride >= (q_len - 1) * out_stride + q_heads * head_dim, "%s: the batch's outputs overlap", name);
-    KREA2_REQUIRE(!key_mask || mask_stride >= kv_len, "%s: mask_stride %zu is below kv_len %zu", name, mask_stride, kv_len);
+    KREA2_REQUIRE(batch == 1 || out_batch_stride >= (q_len - 1) * out_stride + q_heads * head_dim ||
+                      (out_batch_stride >= q_heads * head_dim && out_stride >= (batch - 1) * out_batch_stride + q_heads * head_dim),
+                  "%s: the batch's outputs overlap", name);
+    KREA2_REQUIRE(!key_mask || batch == 1 || mask_stride == 0 || mask_stride >= kv_len, "%s: mask_stride %zu is below kv_len %zu", name, mask_stride, kv_len);
     KREA2_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: scale must be a positive number", name);
     KREA2_REQUIRE(kind == KREA2_F16 || kind == KREA2_BF16, "%s: kind %d is neither KREA2_F16 nor KREA2_BF16", name, kind);
     KREA2_REQUIRE(q && out && (kv_len == 0 || (k && v)), "%s: null buffer", name);

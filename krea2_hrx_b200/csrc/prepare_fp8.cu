@@ -277,6 +277,8 @@ extern "C" int krea2_prepare_norm_fp8(krea2_stream stream, size_t tokens, const 
     KREA2_REQUIRE(residual || !sum, "%s: a sum is written only where there is a residual", name);
     KREA2_REQUIRE(!residual || residual_stride >= width, "%s: residual_stride %zu is below the width %zu", name, residual_stride, width);
     KREA2_REQUIRE(!sum || sum_stride >= width, "%s: sum_stride %zu is below the width %zu", name, sum_stride, width);
+    KREA2_REQUIRE((sum != x || sum_stride == x_stride) && (!sum || sum != residual || sum_stride == residual_stride),
+                  "%s: a sum in place needs the stride of the buffer that it replaces", name);
     KREA2_REQUIRE(reinterpret_cast<uintptr_t>(residual) % 2 == 0 && reinterpret_cast<uintptr_t>(sum) % 2 == 0 &&
                       reinterpret_cast<uintptr_t>(weight) % 4 == 0,
                   "%s: buffers must be aligned to their element size", name);

@@ -1,5 +1,9 @@
 """Cross attention against its definition in 64 bits: lengths, masks, head layouts, pitches, what lies in keys that do not
 count; and a cross-attention sublayer of all the operators together."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -7,6 +11,8 @@ import operator_definitions as defs
 from operator_definitions import KINDS
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 k = pytest.importorskip("krea2_hrx_b200")
 from krea2_hrx_b200 import ops  # noqa: E402
@@ -106,6 +112,68 @@ def test_views_of_wider_tensors_and_shared_states(q_len):
     out = torch.empty((3, q_len, 4, 64), dtype=torch.bfloat16, device="cuda")
     ops.cross_attention(q, key, value, out)
     defs.check_cross(out, q, key, value, 0.125)
+
+
+@pytest.mark.parametrize("q_len", [1, 150])
+def test_sequence_first_layouts_and_a_shared_mask(q_len):
+    """[length][batch][heads][dim] tensors seen batch first, outputs too; one mask for the whole batch, one query for all."""
+    q, key, value = (rows_of(n, 3, h, 64, torch.float16, n).transpose(0, 1) for n, h in ((q_len, 4), (300, 2), (301, 2)))
+    value = value[:, :300]
+    out = torch.full((q_len + 1, 3, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    mask = (torch.rand(300, generator=torch.Generator().manual_seed(1)) < 0.5).expand(3, 300)
+    ops.cross_attention(q, key, value, out[:q_len].transpose(0, 1), key_mask=mask.cuda()[:1].expand(3, 300))
+    defs.check_cross(out[:q_len].transpose(0, 1), q, key, value, 0.125, key_mask=mask)
+    assert bool((out[q_len] == 7.0).all())
+    shared = q[:1].expand(3, q_len, 4, 64)
+    again = torch.empty((3, q_len, 4, 64), dtype=torch.float16, device="cuda")
+    ops.cross_attention(shared, key, value, again)
+    defs.check_cross(again, shared, key, value, 0.125)
+
+
+@pytest.mark.parametrize("heads", [3, 5, 7, 24, 128])
+def test_heads_that_do_not_fill_a_tile(heads):
+    """Row tiles of 128 // heads queries: the rows left over in a tile belong to nobody."""
+    attend(2, 100, 200, heads, 1, 64, torch.bfloat16, lengths=[200, 77])
+
+
+def test_first_calls_inside_a_capture(tmp_path):
+    """A process whose first call of every operator is recorded into a graph."""
+    script = tmp_path / "capture.py"
+    script.write_text(f"""
+import sys
+sys.path[:0] = [{ROOT!r}, {os.path.join(ROOT, 'tests')!r}]
+import torch
+import operator_definitions as defs
+from krea2_hrx_b200 import ops
+g = torch.Generator().manual_seed(0)
+t = lambda *shape: torch.randn(shape, generator=g).to(torch.bfloat16).cuda()
+codes = lambda m, k: torch.empty((m, k), dtype=torch.float8_e4m3fn, device="cuda")
+x, w, out = t(300, 512), t(384, 512), torch.empty((300, 384), dtype=torch.bfloat16, device="cuda")
+a, a_scale, b, b_scale = codes(300, 512), torch.empty((300, 4), device="cuda"), codes(384, 512), torch.ones((3, 4), device="cuda")
+b.view(torch.uint8).copy_(w.to(torch.float8_e4m3fn).view(torch.uint8))
+small = torch.empty((5, 384), dtype=torch.bfloat16, device="cuda")
+q, kv, o = t(2, 50, 4, 64), t(2, 70, 2, 64), torch.empty((2, 50, 4, 64), dtype=torch.bfloat16, device="cuda")
+f, _ = ops.rotary_frequencies(64)
+r = torch.empty((100, 4, 64), dtype=torch.bfloat16, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.prepare_norm_fp8(x, None, a, a_scale, weight_offset=1.0)
+    ops.gemm_fp8_128(a, a_scale, b, b_scale, out)
+    ops.gemm_fp8_128(a[:5], a_scale[:5], b, b_scale, small)
+    ops.rotary(q.view(100, 4, 64), None, r, None, f)
+    ops.cross_attention(q, kv, kv, o)
+graph.replay()
+torch.cuda.synchronize()
+defs.check_codes(a, a_scale, defs.norm_rows(x, None, None, 1e-5, 1.0)[0], 60)
+defs.check_product(out, a, a_scale, b, b_scale)
+defs.check_product(small, a.view(torch.uint8)[:5].view(a.dtype), a_scale[:5], b, b_scale)
+defs.check_rotary(r, q.view(100, 4, 64), torch.arange(100), f, 1.0, "interleaved", False)
+defs.check_cross(o, q, kv, kv, 0.125)
+print("captured")
+""")
+    done = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
 
 
 @pytest.mark.parametrize("q_len", [2, 300])

@@ -51,6 +51,10 @@ REFUSED = [
     ("krea2_cross_attention", dict(head_dim=60), "head_dim"), ("krea2_cross_attention", dict(q_stride=248), "strides"),
     ("krea2_cross_attention", dict(k_stride=120), "strides"), ("krea2_cross_attention", dict(v_stride=132), "multiples of 8"),
     ("krea2_cross_attention", dict(k_batch_stride=900), "multiples of 8"), ("krea2_cross_attention", dict(out_batch_stride=256), "overlap"),
+    ("krea2_prepare_norm_fp8", dict(residual="p+16", residual_stride=256, sum="p", sum_stride=512), "in place"),
+    ("krea2_prepare_norm_fp8", dict(residual="p+16", residual_stride=256, sum="p+16", sum_stride=512), "in place"),
+    ("krea2_cross_attention", dict(q_heads=258, head_dim=8, q_stride=2064, out_stride=2064, q_batch_stride=16384, out_batch_stride=16384), "share a key head"),
+    ("krea2_cross_attention", dict(out_batch_stride=0), "overlap"), ("krea2_cross_attention", dict(out_batch_stride=248, out_stride=512), "overlap"),
     ("krea2_cross_attention", dict(key_mask="p", mask_stride=6), "mask_stride"), ("krea2_cross_attention", dict(scale=0.0), "scale"),
     ("krea2_cross_attention", dict(scale=float("nan")), "scale"), ("krea2_cross_attention", dict(scale=-1.0), "scale"),
     ("krea2_cross_attention", dict(kind=2), "kind"), ("krea2_cross_attention", dict(v=None), "null"), ("krea2_cross_attention", dict(q="p+8"), "aligned"),
