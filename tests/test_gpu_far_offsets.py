@@ -47,7 +47,7 @@ def test_codes_and_product(store):
         ops.gemm_fp8_128(codes, scales, w, w_scale, c)
         defs.check_product(c, codes.view(torch.uint8).contiguous().view(codes.dtype), scales, w, w_scale)
     # many rows of a: the last ones' outputs lie behind 2^31 elements
-    rows = 16400
+    rows = 16380
     a, a_scale = ops.QuantizedFp8(seeded(rows, 320)).weight, torch.rand((rows, 3), device="cuda")
     c = store[0].as_strided((rows, 200), (2 ** 18 + 8, 1))
     ops.gemm_fp8_128(a, a_scale, w, w_scale, c)
