@@ -86,9 +86,9 @@ __device__ __forceinline__ float block_sum(float v, float *shared) {
 // the codes.  HBM-bound: a block walks rows gridDim.x apart and requests the next one before it works on the present one
 // (not the widest rows, whose values fill the registers).
 template <bool kBf16, bool kNorm, bool kResidual, bool kVector, int kPer>
-__global__ void __launch_bounds__(kPer == 1 ? 1024 : kPer == 2 ? 256 : 512, kPer == 2 ? 3 : 1)
+__global__ void __launch_bounds__(kPer <= 2 ? 1024 : kPer == 3 ? 256 : 512, kPer == 3 ? 4 : 1)
 prepare_fp8_kernel(const PrepareArgs g) {
-    constexpr bool kAhead = kVector && kPer <= 4;  // single elements are packed as they arrive: asking early would wait for them
+    constexpr bool kAhead = kVector && kPer <= 3;  // single elements are packed as they arrive: asking early would wait for them
     __shared__ float partial[2][32];
     const bool wide_weight = kVector && (reinterpret_cast<uintptr_t>(g.weight) & 15u) == 0u;
     uint4 x[kPer], residual[kResidual ? kPer : 1];
@@ -213,17 +213,17 @@ int launch_runs(cudaStream_t stream, const PrepareArgs &g, uint32_t runs) {
     return KREA2_OK;
 }
 
-// Few rows: one run a thread, for the latency (3.6 us for 148 rows of 6144).  Many: two to four, so that several blocks share
-// an SM and one's loads run under another's sums (4608 rows of 6144 and their residual take 70 us with one run a thread and
-// a block per row).
+// Few rows (or narrow ones): one run a thread, for the latency (2.8 us for one row of 6144).  Many: two or three, so that
+// four blocks of up to 256 threads share an SM and one's loads run under another's sums: 4608 rows of 6144 and their
+// residual take 38 us (80 % of the HBM rate, 89 % for 16896 rows), 70 us with one run a thread and a block per row.  Wider
+// rows: two runs in up to 1024 threads, 28 us for 1043 rows of 16384 and their residual, 32 us with four runs in 512.
 template <bool kBf16, bool kNorm, bool kResidual, bool kVector>
 int launch_prepare(cudaStream_t stream, const PrepareArgs &g) {
     const uint32_t runs = (g.width + 7) / 8;
     if (runs <= 1024 && (!kVector || g.tokens <= static_cast<uint32_t>(multiprocessors()) || runs <= 128))
         return launch_runs<kBf16, kNorm, kResidual, kVector, 1>(stream, g, runs);
-    if (runs <= 512) return launch_runs<kBf16, kNorm, kResidual, kVector, 2>(stream, g, runs);
-    if (runs <= 1536) return launch_runs<kBf16, kNorm, kResidual, kVector, 3>(stream, g, runs);
-    if (runs <= 2048) return launch_runs<kBf16, kNorm, kResidual, kVector, 4>(stream, g, runs);
+    if (runs > 512 && runs <= 768) return launch_runs<kBf16, kNorm, kResidual, kVector, 3>(stream, g, runs);
+    if (runs <= 2048) return launch_runs<kBf16, kNorm, kResidual, kVector, 2>(stream, g, runs);
     return launch_runs<kBf16, kNorm, kResidual, kVector, 8>(stream, g, runs);
 }
 
