@@ -100,6 +100,18 @@ __device__ __forceinline__ uint16_t bits_of(float v) {
     return kBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
+// Two f32 as a pair of bf16 or f16 patterns, the first in the low half.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if constexpr (kBf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
 // exp with a fixed evaluation order: Cody-Waite reduction by ln 2 in two pieces, the degree-6
 // Cephes polynomial, scaling by two exact powers of two.  It stands in for the reference's
 // approximate `expf<afn>` (kernels/prepare_gated_i8.loom:99, gemm_i8_swiglu_256.loom:650).

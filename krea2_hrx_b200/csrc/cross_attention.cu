@@ -53,16 +53,6 @@ struct Cross {
     static_assert(2 * (kSharedBytes + 1024) <= 228 * 1024 && 3 * kSharedBytes > 228 * 1024, "two CTAs share an SM and its tensor memory");
 };
 
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
-    if constexpr (kBf16) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __half2 v = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -33,10 +33,6 @@ struct ProductArgs {
     uint32_t panels;  // wide kernel: column tiles walked together (0: a column of tiles top to bottom)
 };
 
-__device__ __forceinline__ uint32_t pack_outputs(float lo, float hi, uint32_t bf16) {
-    if (bf16) return bits_of<true>(lo) | (static_cast<uint32_t>(bits_of<true>(hi)) << 16);
-    return bits_of<false>(lo) | (static_cast<uint32_t>(bits_of<false>(hi)) << 16);
-}
 
 // kind::f8f6f4: f32 accumulate (1 at bit 4), e4m3 A and B (0 at bits 7 and 10), both K-major, N/8 at bit 17, M/16 at bit 24.
 __host__ __device__ constexpr uint32_t product_descriptor(int m, int n) {
@@ -140,26 +136,36 @@ struct Wide {
 
 // Writes 32 outputs of each of the warp's 32 rows through its staging area, so that rows leave in 64-byte pieces; the
 // 16-byte pieces of a row change places from one pair of rows to the next, which spreads a column of them over the banks.
+template <bool kBf16>
 __device__ __forceinline__ void store_wide(const ProductArgs &g, const float2 *values, uint32_t row0, uint32_t column0, uint8_t *staging, int lane) {
     auto piece = [&](uint32_t row, uint32_t i) { return staging + row * 64 + ((i ^ ((row >> 1) & 3u)) * 16); };
 #pragma unroll
     for (uint32_t i = 0; i < 4; i++)
         *reinterpret_cast<uint4 *>(piece(lane, i)) =
-            make_uint4(pack_outputs(values[4 * i].x, values[4 * i].y, g.bf16), pack_outputs(values[4 * i + 1].x, values[4 * i + 1].y, g.bf16),
-                       pack_outputs(values[4 * i + 2].x, values[4 * i + 2].y, g.bf16), pack_outputs(values[4 * i + 3].x, values[4 * i + 3].y, g.bf16));
+            make_uint4(pack_pair<kBf16>(values[4 * i].x, values[4 * i].y), pack_pair<kBf16>(values[4 * i + 1].x, values[4 * i + 1].y),
+                       pack_pair<kBf16>(values[4 * i + 2].x, values[4 * i + 2].y), pack_pair<kBf16>(values[4 * i + 3].x, values[4 * i + 3].y));
     __syncwarp();
     if (g.aligned) {
-        const uint32_t column = column0 + (lane & 3) * 8;
+        const uint32_t column = column0 + (lane & 3) * 8, row = row0 + (lane >> 2);
+        uint4 v[4];
 #pragma unroll
-        for (int r = 0; r < 32; r += 8) {
-            const uint32_t local = r + (lane >> 2), row = row0 + local;
-            if (row >= g.m || column >= g.n) continue;
-            const uint8_t *from = piece(local, lane & 3);
-            uint16_t *to = g.c + row * g.c_stride + column;
-            if (column + 8 <= g.n) {
-                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
-            } else {
-                for (uint32_t i = 0; column + i < g.n; i++) to[i] = reinterpret_cast<const uint16_t *>(from)[i];
+        for (int r = 0; r < 4; r++) v[r] = *reinterpret_cast<const uint4 *>(piece(8 * r + (lane >> 2), lane & 3));
+        uint16_t *to = g.c + row * g.c_stride + column;
+        if (row0 + 32 <= g.m && column0 + 32 <= g.n) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) *reinterpret_cast<uint4 *>(to + 8 * r * g.c_stride) = v[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if (row + 8 * r >= g.m) continue;
+                if (column + 8 <= g.n) {
+                    *reinterpret_cast<uint4 *>(to + 8 * r * g.c_stride) = v[r];
+                } else {
+                    const uint32_t words[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (column + i < g.n) to[8 * r * g.c_stride + i] = static_cast<uint16_t>(words[i >> 1] >> (16 * (i & 1)));
+                }
             }
         }
     } else if (column0 + lane < g.n) {
@@ -169,6 +175,7 @@ __device__ __forceinline__ void store_wide(const ProductArgs &g, const float2 *v
     __syncwarp();
 }
 
+template <bool kBf16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide::kThreads, 1)
 wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const ProductArgs g) {
     using T = Wide;
@@ -345,7 +352,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             if (!alive) break;
 #pragma unroll
             for (int c = 0; c < T::kWarpColumns / 32; c++)
-                store_wide(g, out + c * 16, row0, column0 + c * 32, staging + warp * T::kStagingBytes, lane);
+                store_wide<kBf16>(g, out + c * 16, row0, column0 + c * 32, staging + warp * T::kStagingBytes, lane);
         }
     }
 
@@ -585,7 +592,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 #pragma unroll
         for (uint32_t r = 0; r < 8; r++)
             if (r < shares) total.x += share[r].x, total.y += share[r].y, total.z += share[r].z, total.w += share[r].w;
-        const uint2 packed = make_uint2(pack_outputs(total.x, total.y, g.bf16), pack_outputs(total.z, total.w, g.bf16));
+        const uint2 packed = g.bf16 ? make_uint2(pack_pair<true>(total.x, total.y), pack_pair<true>(total.z, total.w))
+                                    : make_uint2(pack_pair<false>(total.x, total.y), pack_pair<false>(total.z, total.w));
         uint16_t *to = g.c + (m0 + token) * g.c_stride + column;
         if (g.aligned && column + 4 <= g.n) {
             *reinterpret_cast<uint2 *>(to) = packed;
@@ -676,10 +684,11 @@ int launch_narrow(cudaStream_t stream, const void *a, const void *w, size_t k, s
     return KREA2_OK;
 }
 
+template <bool kBf16>
 int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, ProductArgs g) {
     using T = Wide;
     static Prepared prepared;
-    if (int status = prepare_kernel(prepared, wide_kernel, T::kSharedBytes)) return status;
+    if (int status = prepare_kernel(prepared, wide_kernel<kBf16>, T::kSharedBytes)) return status;
     CUtensorMap map_a, map_w;
     if (int status = operand_map(&map_a, a, g.m, k, a_stride, T::kRows)) return status;
     if (int status = operand_map(&map_w, w, g.n, k, w_stride, T::kRows / 2)) return status;
@@ -692,16 +701,16 @@ int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, siz
     }
     const uint32_t tiles = ((g.m + 2 * T::kRows - 1) / (2 * T::kRows)) * ((g.n + T::kColumns - 1) / T::kColumns);
     const uint32_t pairs = static_cast<uint32_t>(multiprocessors()) / 2;
-    wide_kernel<<<2 * (tiles < pairs ? tiles : pairs), T::kThreads, T::kSharedBytes, stream>>>(map_a, map_w, g);
+    wide_kernel<kBf16><<<2 * (tiles < pairs ? tiles : pairs), T::kThreads, T::kSharedBytes, stream>>>(map_a, map_w, g);
     const cudaError_t status = cudaGetLastError();
     if (status != cudaSuccess) return fail(KREA2_RUNTIME, "gemm_fp8_128 launch failed: %s", cudaGetErrorString(status));
     return KREA2_OK;
 }
 
-// The kernel and tile that are expected to take least.  The wide kernel takes 8 us and, for each round of tiles over the
-// pairs of SMs, 0.44 us a block.  It has the rows that fill its tiles: of 6144 columns and channels it takes 29 us for 128 to
-// 512 rows and 31 for 768, the narrow one (its best tile) 14 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512 and 47
-// for 768.  Beyond 1024 rows no shape's estimate chooses the narrow one.
+// The kernel and tile that are expected to take least.  The wide kernel takes 7.5 us and, for each round of tiles over the
+// pairs of SMs, 1 us and 0.4 us a block.  It has the rows that fill its tiles: of 6144 columns and channels it takes 26 us for
+// 128 to 512 rows and 29 for 768, the narrow one (its best tile) 14 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512
+// and 47 for 768.  Beyond 1024 rows no shape's estimate chooses the narrow one.
 int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, const ProductArgs &g) {
     NarrowPlan plan;
 #define KREA2_NARROW(tokens)                                                                       \
@@ -715,7 +724,7 @@ int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, 
     if (g.m <= 1024) {
         const uint32_t tiles = ((g.m + 2 * Wide::kRows - 1) / (2 * Wide::kRows)) * ((g.n + Wide::kColumns - 1) / Wide::kColumns);
         const uint32_t pairs = static_cast<uint32_t>(multiprocessors()) / 2;
-        float least = ((tiles + pairs - 1) / pairs) * (0.44f * g.blocks + 1.0f) + 8.0f;
+        float least = ((tiles + pairs - 1) / pairs) * (0.40f * g.blocks + 1.0f) + 7.5f;
         int tokens = 0;
         uint32_t shares = 1;
 #define KREA2_NARROW(candidate)                                                                    \
@@ -739,7 +748,7 @@ int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, 
             default: break;
         }
     }
-    return launch_wide(stream, a, w, k, a_stride, w_stride, g);
+    return g.bf16 ? launch_wide<true>(stream, a, w, k, a_stride, w_stride, g) : launch_wide<false>(stream, a, w, k, a_stride, w_stride, g);
 }
 
 }  // namespace
