@@ -114,8 +114,7 @@ prepare_fp8_kernel(const PrepareArgs g) {
                 unpack8<kBf16>(residual[j], other);
                 uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w[i] = bits_of<kBf16>(v[j][2 * i] + other[2 * i]) | (static_cast<uint32_t>(bits_of<kBf16>(v[j][2 * i + 1] + other[2 * i + 1])) << 16);
+                for (int i = 0; i < 4; i++) w[i] = pack_pair<kBf16>(v[j][2 * i] + other[2 * i], v[j][2 * i + 1] + other[2 * i + 1]);
                 const uint4 total = make_uint4(w[0], w[1], w[2], w[3]);
                 unpack8<kBf16>(total, v[j]);
                 if (g.sum != nullptr) store8<kVector>(g.sum + row * g.sum_stride, run_of(j), g.width, total);

@@ -40,11 +40,6 @@ template <bool kBf16>
 __device__ __forceinline__ float low_value(uint32_t word) { return value_of<kBf16>(static_cast<uint16_t>(word)); }
 template <bool kBf16>
 __device__ __forceinline__ float high_value(uint32_t word) { return value_of<kBf16>(static_cast<uint16_t>(word >> 16)); }
-template <bool kBf16>
-__device__ __forceinline__ uint32_t word_of(float lo, float hi) {
-    return bits_of<kBf16>(lo) | (static_cast<uint32_t>(bits_of<kBf16>(hi)) << 16);
-}
-
 // HBM-bound.  A warp walks heads of one token, four heads' loads in flight (the first are under way before the angles are
 // taken); `warps` warps share a token's heads where the tokens do not fill the device.  The token's cosines and sines are
 // taken once per warp, a pair per lane, and lie in shared memory; a lane keeps those of its piece in registers.
@@ -110,14 +105,14 @@ rotary_pieces_kernel(const RotaryArgs g, uint32_t tokens, uint32_t warps) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float p = low_value<kBf16>(own[i]), q = high_value<kBf16>(own[i]);
-                        if (i < inside) own[i] = word_of<kBf16>(p * by[i].x - q * by[i].y, q * by[i].x + p * by[i].y);
+                        if (i < inside) own[i] = pack_pair<kBf16>(p * by[i].x - q * by[i].y, q * by[i].x + p * by[i].y);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t other = __shfl_sync(0xffffffffu, own[i], partner & 31u);
                         const float2 c0 = by[2 * i], c1 = by[2 * i + 1];
-                        const uint32_t turned = word_of<kBf16>(low_value<kBf16>(own[i]) * c0.x + low_value<kBf16>(other) * c0.y,
+                        const uint32_t turned = pack_pair<kBf16>(low_value<kBf16>(own[i]) * c0.x + low_value<kBf16>(other) * c0.y,
                                                                high_value<kBf16>(own[i]) * c1.x + high_value<kBf16>(other) * c1.y);
                         if (inside) own[i] = turned;  // a channel that is not turned is copied, whatever it holds
                     }
