@@ -6,10 +6,16 @@
 //
 // One pass over the keys with a running maximum and sum.  A CTA owns up to 128 rows of one key head: the query heads that
 // share it are packed (row r is query r / shares, head r % shares of the key head's), so a single query fills as many rows as
-// heads share its keys, and one tile load or store moves the rows of 128 / shares queries.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with f32 accumulators in tensor memory; K and V
-// tiles of 128 keys arrive by TMA as they lie (V is the second product's B operand with its channels innermost, so nothing
-// is transposed), a thread owns one row's softmax and writes P over S in tensor memory.  Two CTAs share an SM: one's
-// softmax, its start and its output run under the other's products.
+// heads share its keys, and one tile load or store moves the rows of 128 / shares queries.  S = Q K^T and O += P V are
+// tcgen05.mma kind::f16 with f32 accumulators in tensor memory; K and V tiles of 128 keys arrive by TMA as they lie (V is
+// the second product's B operand with its channels innermost, so nothing is transposed), a thread owns one row's softmax
+// and writes P over S in tensor memory.  Two CTAs share an SM: one's softmax, its start and its output run under the
+// other's products.
+//
+// Bound by the chain of a row tile, scores -> softmax -> second product, of which an SM has two under way: 16384 queries of
+// 48/12 heads of 128 to 512 keys take 240-265 us (0.78-0.86 PFLOP/s: four key tiles a CTA, so its start and end weigh), 4608
+// to 4608 480 us (1.09 PFLOP/s, tensor pipe 0.5 active).  Heads of 64 do half the products for the same exponentials and are
+// bound by those; a mask's selects cost 22-30 % more softmax.  One row tile per head of a single query: 7.3 us for 512 keys.
 // Where the rows do not fill the device, a cluster of up to eight CTAs splits the keys of a row tile and adds its partial
 // outputs over distributed shared memory in the order of their rank: no workspace, the same bits every time.
 #include <atomic>
@@ -24,6 +30,13 @@ __device__ int g_cross_status = 0;  // folded into krea2_device_status by take_c
 constexpr int kCrossTimedOut = 128;
 
 constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
+
+// Weights are rounded to the tensors' type for the second product (half a step each; their sum is taken before).  A weight
+// far below its row's largest would be lost in f16, whose numbers end at 2^-25, and many such may count, so f16 weights
+// carry a factor of 2^7, which drops out with the sum: the largest is 2^15 (the reference lags by 2^8 at most), and what is
+// 2^-32 of the reference still counts.
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 0.0f : 7.0f;
 
 struct CrossArgs {
     const int32_t *kv_lengths;
@@ -367,7 +380,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 tensor_stores_done();
             }
-            const float shift = reference == -INFINITY ? 0.0f : -reference;  // nothing counted yet: the weights are zero, not NaN
+            const float shift = reference == -INFINITY ? 0.0f : kLift<kBf16> - reference;  // nothing counted yet: the weights are zero, not NaN
             float2 total[4];
 #pragma unroll
             for (int t = 0; t < 4; t++) total[t] = make_float2(0.0f, 0.0f);

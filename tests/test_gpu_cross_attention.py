@@ -1,5 +1,6 @@
 """Cross attention against its definition in 64 bits: lengths, masks, head layouts, pitches, what lies in keys that do not
 count; and a cross-attention sublayer of all the operators together."""
+import math
 import os
 import subprocess
 import sys
@@ -85,6 +86,24 @@ def test_large_scores_and_another_scale():
     out = torch.empty_like(q)
     ops.cross_attention(q, key, value, out)
     defs.check_cross(out, q, key, value, 0.125)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("q_len,kv_len", [(1, 16384), (1000, 4096)])
+def test_many_small_weights_count(kind, q_len, kv_len):
+    """One key takes nearly all of a row, the others 2^-26 of it each and carry the only values: rounded on their own for the
+    second product, they must not vanish."""
+    dtype = KINDS[kind]
+    q, key = torch.zeros((1, q_len, 2, 64), dtype=dtype, device="cuda"), torch.zeros((1, kv_len, 2, 64), dtype=dtype, device="cuda")
+    q[..., 0], key[:, 1:, :, 0], value = 1.0, -26.0, torch.ones_like(key)
+    value[:, 0] = 0.0
+    out = torch.empty_like(q)
+    ops.cross_attention(q, key, value, out, scale=math.log(2.0))
+    small = (kv_len - 1) * 2.0 ** -26
+    # 2^-26 is a power of two, which a weight that is off by its f32 arguments' rounding (26 * 2^-23 at most) rounds to; the
+    # output is rounded once.
+    want, eps = small / (1.0 + small), torch.finfo(dtype).eps / 2
+    assert float((out.double() - want).abs().max()) <= want * (eps + 1e-5)
 
 
 def test_no_keys_at_all():
