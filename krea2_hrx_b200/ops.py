@@ -381,6 +381,7 @@ class QuantizedFp8:
         if weight.dim() != 2 or not weight.is_floating_point() or not weight.is_cuda or 0 in weight.shape:
             raise InvalidArgument("an e4m3 projection takes a floating CUDA weight [outputs][inputs]")
         self.outputs, self.inputs = weight.shape
+        weight = weight.detach()
         rows, columns = _groups(self.outputs), _groups(self.inputs)
         blocks = torch.zeros((rows * GROUP, columns * GROUP), dtype=torch.float32, device=weight.device)
         blocks[: self.outputs, : self.inputs] = weight

@@ -225,6 +225,15 @@ def test_projection(kind):
         layer.forward(x[:, :999])
 
 
+def test_projection_of_a_weight_that_is_trained():
+    """A projection is a copy in codes: it keeps no graph of the weight that it was made from."""
+    weight = torch.randn((40, 300), generator=torch.Generator().manual_seed(2)).cuda().requires_grad_()
+    layer, plain = ops.QuantizedFp8(weight), ops.QuantizedFp8(weight.detach())
+    assert not layer.scales.requires_grad and not layer.weight.requires_grad
+    x = rows_of(5, 300, torch.bfloat16, 3)
+    assert torch.equal(layer.forward(x), plain.forward(x))
+
+
 def test_shape_and_type_refusals():
     t = torch.zeros((4, 128), dtype=torch.bfloat16, device="cuda")
     q, scale = torch.zeros((4, 128), dtype=E4M3, device="cuda"), torch.zeros((4, 1), device="cuda")
