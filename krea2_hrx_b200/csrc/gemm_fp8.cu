@@ -33,7 +33,6 @@ struct ProductArgs {
     uint32_t panels;  // wide kernel: column tiles walked together (0: a column of tiles top to bottom)
 };
 
-
 // kind::f8f6f4: f32 accumulate (1 at bit 4), e4m3 A and B (0 at bits 7 and 10), both K-major, N/8 at bit 17, M/16 at bit 24.
 __host__ __device__ constexpr uint32_t product_descriptor(int m, int n) {
     return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
@@ -115,6 +114,11 @@ struct ScaleRing {
 };
 
 // ---------------------------------------------------------------- wide
+// Bound by what the block scales cost: a block's four products take 512 clocks of the pair's tensor cores, but its 256 x 256
+// sums also leave tensor memory and pass through the FMA pipes each time, and the two get in each other's way: 735 clocks a
+// block.  4608 x 15360 x 6144 takes 409-445 us (2.0-2.1 PFLOP/s, 0.6 of the e4m3 rate; 1.5 GHz at the power cap).  With an
+// eighth of the sums read it took 341 us, with a quarter of the products 346, with both 228.  Sixteen epilogue warps, loads
+// of 32 columns, one product of 256 columns instead of two of 128: no faster.
 struct Wide {
     static constexpr int kRows = 128;     // of a, and of w, per CTA
     static constexpr int kColumns = 256;  // of a tile
@@ -391,6 +395,9 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ---------------------------------------------------------------- narrow
+// One row: bound by HBM once the weights are large (15360 x 16384: 50 us, 5.05 TB/s), by the start, the ramp of the loads and
+// the addition of the shares below (6144 x 6144: 11.2 us against 5.9 for the bytes).  A few hundred rows: by what the tiles
+// take out of L2, 13-15 TB/s (275 x 6144 x 16384: 43 us).
 constexpr int power_of_two(int n) { return n <= 32 ? 32 : 2 * power_of_two((n + 1) / 2); }
 
 template <int kTokens>

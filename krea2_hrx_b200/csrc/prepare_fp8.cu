@@ -221,7 +221,8 @@ int launch_prepare(cudaStream_t stream, const PrepareArgs &g) {
     const uint32_t runs = (g.width + 7) / 8;
     if (runs <= 1024 && (!kVector || g.tokens <= static_cast<uint32_t>(multiprocessors()) || runs <= 128))
         return launch_runs<kBf16, kNorm, kResidual, kVector, 1>(stream, g, runs);
-    if (runs > 512 && runs <= 768) return launch_runs<kBf16, kNorm, kResidual, kVector, 3>(stream, g, runs);
+    if constexpr (kVector)
+        if (runs > 512 && runs <= 768) return launch_runs<kBf16, kNorm, kResidual, kVector, 3>(stream, g, runs);
     if (runs <= 2048) return launch_runs<kBf16, kNorm, kResidual, kVector, 2>(stream, g, runs);
     return launch_runs<kBf16, kNorm, kResidual, kVector, 8>(stream, g, runs);
 }

@@ -4,6 +4,7 @@
 
 #include <cuda.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "common.cuh"
@@ -331,15 +332,15 @@ inline int make_tensor_map(CUtensorMap *map, CUtensorMapDataType type, uint32_t 
 
 // The current device's number of SMs.
 inline int multiprocessors() {
-    static int cached[64];
+    static std::atomic<int> cached[64];
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 148;
-    if (cached[device] == 0) {
-        int n = 0;
+    int n = cached[device].load(std::memory_order_relaxed);
+    if (n == 0) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
-        cached[device] = n;
+        cached[device].store(n, std::memory_order_relaxed);
     }
-    return cached[device];
+    return n;
 }
 
 // Raises a kernel's dynamic shared-memory limit, once per device and kernel (`once` and `status` belong to the kernel).
