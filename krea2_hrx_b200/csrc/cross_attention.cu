@@ -539,8 +539,12 @@ int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_
     config.numAttrs = 1;
     const uint32_t row_tiles = (g.q_len + g.queries - 1) / g.queries, key_tiles = (g.kv_len + kRows - 1) / kRows;
     const size_t tiles = row_tiles * batch * kv_heads;
-    // The split of the keys that takes least by the measured parts: a tile of keys 1.9 us, a CTA's start and end 4 us, the
-    // addition of the shares 3 us; CTAs beyond those that are resident at once run in further rounds.
+    // The split of the keys that takes least by the measured parts: a tile of keys 2.2 us where two CTAs share an SM and 1.5
+    // where one has it alone (in the last round, if it fills half of the device at most), a CTA's start and end 4 us, or 5 us
+    // and for the addition of the shares 1.6 us a share, less where a row tile is not full.  (4 row tiles of 100 rows to 1000
+    // keys: 17.6 us in one part, 15.3, 13.7, 12.5 in two to four, 13.8 in six or eight; 96 of 128 rows to 4096 keys: 54 in
+    // one, 42 in two, 60 in three.)
+    const float addition = 1.6f / kRows * static_cast<float>((g.q_len < g.queries ? g.q_len : g.queries) * g.shares);
     uint32_t parts = 1;
     float least = INFINITY;
     for (uint32_t more = 1; more <= 8 && more <= (key_tiles ? key_tiles : 1u); more++) {
@@ -549,11 +553,17 @@ int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_
             config.gridDim = dim3(more, 1, 1);
             attribute.val.clusterDim.x = more;
             KREA2_CUDA(cudaOccupancyMaxActiveClusters(&clusters, cross_attention_kernel<kD, kBf16>, &config));
-            if (clusters < 1) clusters = 1;
+            // The query counts the registers that the softmax holds after the exchange for every thread, and so one CTA an SM;
+            // two are launched.  (24 row tiles of 600 queries to 4096 keys in two parts, 43 us; in one, as if they did not
+            // fit, 52.)
+            clusters = clusters < 1 ? 2 : 2 * clusters;
             known[device][more].store(clusters, std::memory_order_relaxed);
         }
-        const float rounds = static_cast<float>((tiles + clusters - 1) / clusters);
-        const float time = rounds * (1.9f * static_cast<float>((key_tiles + more - 1) / more) + (more > 1 ? 7.0f : 4.0f));
+        const uint32_t resident = static_cast<uint32_t>(clusters);
+        const float walk = static_cast<float>((key_tiles + more - 1) / more), ends = more > 1 ? 5.0f + addition * static_cast<float>(more) : 4.0f;
+        const float shared = 2.2f * walk + ends, alone = 1.5f * walk + ends;
+        const size_t rest = tiles % resident;
+        const float time = static_cast<float>(tiles / resident) * shared + (rest == 0 ? 0.0f : 2 * rest <= resident ? alone : shared);
         if (time < least) least = time, parts = more;
     }
     attribute.val.clusterDim.x = parts;
