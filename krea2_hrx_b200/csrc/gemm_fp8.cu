@@ -7,7 +7,7 @@
 // Two kernels:
 //   wide    a pair of CTAs owns 256 rows of a and 256 of w (as the int8 pair kernel does); an epilogue thread owns one row
 //           and 128 outputs, whose scale of a block is one number
-//   narrow  few rows of a: 128 rows of w are the M side and up to 256 rows of a the N side of a CTA, the blocks of 128
+//   narrow  few rows of a: 128 rows of w are the M side and up to 192 rows of a the N side of a CTA, the blocks of 128
 //           channels are split over a cluster of up to eight CTAs, whose partial outputs are added over distributed shared
 //           memory in the order of their rank: no workspace, no atomics, the same bits every time
 #include <atomic>
@@ -403,7 +403,7 @@ constexpr int power_of_two(int n) { return n <= 32 ? 32 : 2 * power_of_two((n + 
 template <int kTokens>
 struct Narrow {
     static constexpr int kRows = 128;                        // of w
-    static constexpr int kWarps = kTokens <= 32 ? 4 : kTokens <= 192 ? 8 : 16;  // epilogue
+    static constexpr int kWarps = kTokens <= 32 ? 4 : 8;  // epilogue
     static constexpr int kThreads = (kWarps + 4) * 32;       // and one warp that loads, one that issues, two that lay out scales
     using Scales = ScaleRing<kTokens, true>;
     static constexpr int kColumns = kTokens / (kWarps / 4);  // tokens of one epilogue thread
@@ -643,7 +643,7 @@ struct NarrowPlan {
 };
 
 // The split of the blocks that keeps all clusters resident (more CTAs than that run in a second round, which costs more
-// than the shorter first one saves: 1 x 6144 x 6144 takes 10.6 us in four shares, 15.8 in six), and its time from
+// than the shorter first one saves: 1 x 6144 x 6144 takes 11 us in four shares, 15.8 in six), and its time from
 // measured parts: a CTA's start and end 5 us, a block 0.18 us + 1.65 ns a token (a third more where two CTAs share an SM
 // that is full), and no less than its tiles take out of L2 at 13 TB/s.
 template <int kTokens>
@@ -716,7 +716,7 @@ int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, siz
 
 // The kernel and tile that are expected to take least.  The wide kernel takes 7.5 us and, for each round of tiles over the
 // pairs of SMs, 1 us and 0.4 us a block.  It has the rows that fill its tiles: of 6144 columns and channels it takes 26 us for
-// 128 to 512 rows and 29 for 768, the narrow one (its best tile) 14 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512
+// 128 to 512 rows and 29 for 768, the narrow one (its best tile) 16 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512
 // and 47 for 768.  Beyond 1024 rows no shape's estimate chooses the narrow one.
 int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, const ProductArgs &g) {
     NarrowPlan plan;
