@@ -304,9 +304,9 @@ enum { KREA2_F16 = 0, KREA2_BF16 = 1 };
  * x / sqrt(mean(x^2) + eps) * (weight_offset + weight[i]) where x has first become kind(x + residual) if there is a
  * residual (`sum`, if not NULL, receives it: it may be x or residual, with that stride).  weight f32 [width] or NULL for
  * zeros; weight_offset 1 suits weights stored minus one, as this library's checkpoints hold them, 0 plain ones.  A NaN
- * stays a NaN code in its place; an infinity makes its group (after a norm: its place) NaN.  The sum of squares is an
- * f32: rows whose squares leave its range (bf16 beyond 1e19 / sqrt(width)) count as infinitely long.  width 1..32768,
- * out_stride a multiple of 16. */
+ * stays a NaN code in its place; an infinity makes its group (after a norm: its place) NaN.  Rows of any
+ * finite values are normed, also where their squares leave the range of f32; a row of zeros under eps 0 is NaN.  width
+ * 1..32768, out_stride a multiple of 16. */
 int krea2_prepare_norm_fp8(krea2_stream stream, size_t tokens, const void *x, const void *residual, const float *weight,
                            void *sum, void *q, float *q_scale, size_t width, size_t x_stride, size_t residual_stride,
                            size_t sum_stride, size_t out_stride, float eps, float weight_offset, int kind);
