@@ -45,9 +45,21 @@ typedef void *krea2_stream; /* cudaStream_t */
 const char *krea2_last_error(void);
 /* Library version string. */
 const char *krea2_version(void);
-/* Reads and clears the device-side status word the GEMM sets when one of its bounded
+/* Reads and clears the device-side status word that a kernel sets when one of its bounded
  * waits gives up (0 = healthy).  Synchronises the device. */
 int krea2_device_status(int *host_status);
+/* Whose bits those are: the int8 products', the waits for a peer's data, the attention's, the e4m3 product's, the cross
+ * attention's; CHAIN is what the blocks of a session and the sharded chains can raise. */
+enum {
+    KREA2_STATUS_GEMM_I8 = 15,
+    KREA2_STATUS_SHARD_WAIT = 16,
+    KREA2_STATUS_ATTENTION = 32,
+    KREA2_STATUS_CHAIN = 63,
+    KREA2_STATUS_GEMM_FP8 = 64,
+    KREA2_STATUS_CROSS_ATTENTION = 128
+};
+/* The same for the bits of `mask` alone: the others stay for whoever asks for them.  Synchronises the device. */
+int krea2_device_status_of(int mask, int *host_status);
 
 /* ---------------------------------------------------------------- activation prologues */
 

@@ -32,6 +32,13 @@ pub const KREA2_SHARD_PLAIN: c_int = 0;
 pub const KREA2_SHARD_RESID: c_int = 1;
 pub const KREA2_SHARD_SWIGLU: c_int = 2;
 
+pub const KREA2_STATUS_GEMM_I8: c_int = 15;
+pub const KREA2_STATUS_SHARD_WAIT: c_int = 16;
+pub const KREA2_STATUS_ATTENTION: c_int = 32;
+pub const KREA2_STATUS_CHAIN: c_int = 63;
+pub const KREA2_STATUS_GEMM_FP8: c_int = 64;
+pub const KREA2_STATUS_CROSS_ATTENTION: c_int = 128;
+
 pub const KREA2_F16: c_int = 0;
 pub const KREA2_BF16: c_int = 1;
 pub const KREA2_ROTARY_INTERLEAVED: c_int = 0;
@@ -124,6 +131,7 @@ extern "C" {
     pub fn krea2_last_error() -> *const c_char;
     pub fn krea2_version() -> *const c_char;
     pub fn krea2_device_status(host_status: *mut c_int) -> c_int;
+    pub fn krea2_device_status_of(mask: c_int, host_status: *mut c_int) -> c_int;
     pub fn krea2_prepare_norm_i8(stream: krea2_stream, tokens: usize, h: *const c_void, norm_scale: *const f32, mod_scale: *const f32, mod_shift: *const f32, q: *mut c_void, q_scale: *mut f32, width: usize, out_stride: usize, eps: f32) -> c_int;
     pub fn krea2_prepare_gated_i8(stream: krea2_stream, tokens: usize, attn: *const c_void, gate: *const c_void, q: *mut c_void, q_scale: *mut f32, width: usize, out_stride: usize, gate_stride: usize) -> c_int;
     pub fn krea2_prepare_plain_i8(stream: krea2_stream, tokens: usize, h: *const c_void, q: *mut c_void, q_scale: *mut f32, width: usize, out_stride: usize) -> c_int;

@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_size_t, c_uint16, c_uint32, c_uint64, c_void_p
+from typing import Optional
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # KREA2_B200_LIB names another build of the same library (e.g. one compiled with other build-time choices).
@@ -75,6 +76,7 @@ SIGNATURES = {
     "krea2_last_error": (c_char_p, []),
     "krea2_version": (c_char_p, []),
     "krea2_device_status": (c_int, [POINTER(c_int)]),
+    "krea2_device_status_of": (c_int, [c_int, POINTER(c_int)]),
     "krea2_prepare_norm_i8": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_size_t, c_size_t, c_float]),
     "krea2_prepare_gated_i8": (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t,
@@ -217,7 +219,11 @@ def check(status: int) -> None:
         raise _BY_STATUS.get(status, Internal)(message)
 
 
-def device_status() -> int:
+STATUS_CHAIN = 63  # the bits that a session's blocks and the sharded chains can raise (KREA2_STATUS_CHAIN)
+
+
+def device_status(mask: Optional[int] = None) -> int:
+    """Reads and clears the device status word, or the bits of `mask` alone (the others stay); synchronises the device."""
     value = c_int(0)
-    check(lib().krea2_device_status(ctypes.byref(value)))
+    check(lib().krea2_device_status(ctypes.byref(value)) if mask is None else lib().krea2_device_status_of(mask, ctypes.byref(value)))
     return value.value

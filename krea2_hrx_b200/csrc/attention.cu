@@ -1111,14 +1111,7 @@ int ensure_attention() {
 int prepare_attention_device() { return ensure_attention(); }
 
 // Reads and clears the attention kernel's status word (the device is already synchronised).
-int take_attention_status(int *value) {
-    KREA2_CUDA(cudaMemcpyFromSymbol(value, g_attention_status, sizeof(int)));
-    if (*value != 0) {
-        int zero = 0;
-        KREA2_CUDA(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(int)));
-    }
-    return KREA2_OK;
-}
+int take_attention_status(int mask, int *value) { return take_status_bits(g_attention_status, mask, value); }
 
 }  // namespace krea2
 

@@ -36,10 +36,22 @@ void clear_error();
 int prepare_gemm_device();
 // Defined with the attention kernel: the same for it, and its share of the device status word.
 int prepare_attention_device();
-int take_attention_status(int *value);
+int take_attention_status(int mask, int *value);
 // Defined with the e4m3 product and the cross attention: their shares of the status word.
-int take_product_status(int *value);
-int take_cross_status(int *value);
+int take_product_status(int mask, int *value);
+int take_cross_status(int mask, int *value);
+// Reads the bits of `mask` of a kernel file's status word and clears those (the device is already synchronised).
+template <typename Word>
+int take_status_bits(Word &word, int mask, int *value) {
+    int bits = 0;
+    *value = 0;
+    KREA2_CUDA(cudaMemcpyFromSymbol(&bits, word, sizeof(int)));
+    if ((bits & mask) == 0) return KREA2_OK;
+    const int left = bits & ~mask;
+    KREA2_CUDA(cudaMemcpyToSymbol(word, &left, sizeof(int)));
+    *value = bits & mask;
+    return KREA2_OK;
+}
 // Defined with the prologues: their first-use work, for callers about to capture a stream; and
 // prepare_gated_i8 whose attention rows have a pitch of their own (in elements).
 int prepare_prologue_device(cudaStream_t stream);

@@ -27,7 +27,8 @@ namespace krea2 {
 namespace {
 
 __device__ int g_cross_status = 0;  // folded into krea2_device_status by take_cross_status
-constexpr int kCrossTimedOut = 128;
+std::atomic<bool> g_cross_launched{false};  // whether the word is worth a copy: a chain's status reads are not to wait for it
+constexpr int kCrossTimedOut = KREA2_STATUS_CROSS_ATTENTION;
 
 constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
 
@@ -575,13 +576,9 @@ int launch_cross(cudaStream_t stream, const CrossMaps &maps, size_t batch, size_
 
 }  // namespace
 
-int take_cross_status(int *value) {
-    KREA2_CUDA(cudaMemcpyFromSymbol(value, g_cross_status, sizeof(int)));
-    if (*value != 0) {
-        const int zero = 0;
-        KREA2_CUDA(cudaMemcpyToSymbol(g_cross_status, &zero, sizeof(int)));
-    }
-    return KREA2_OK;
+int take_cross_status(int mask, int *value) {
+    *value = 0;
+    return g_cross_launched.load(std::memory_order_relaxed) ? take_status_bits(g_cross_status, mask, value) : KREA2_OK;
 }
 
 }  // namespace krea2
@@ -632,6 +629,7 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
         if (int status = states_map(&maps.v, bf16, v, head_dim, kv_heads, kv_len, v_shared ? 1 : batch, v_stride, v_batch_stride, 1, kRows)) return status;
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    g_cross_launched.store(true, std::memory_order_relaxed);
     if (head_dim <= 64) return bf16 ? launch_cross<64, true>(s, maps, batch, kv_heads, g) : launch_cross<64, false>(s, maps, batch, kv_heads, g);
     return bf16 ? launch_cross<128, true>(s, maps, batch, kv_heads, g) : launch_cross<128, false>(s, maps, batch, kv_heads, g);
 }

@@ -18,7 +18,8 @@ namespace krea2 {
 namespace {
 
 __device__ int g_product_status = 0;  // folded into krea2_device_status by take_product_status
-constexpr int kProductTimedOut = 64;
+std::atomic<bool> g_product_launched{false};  // whether the word is worth a copy: a chain's status reads are not to wait for it
+constexpr int kProductTimedOut = KREA2_STATUS_GEMM_FP8;
 
 constexpr int kBlock = 128;  // channels under one scale = bytes of K per stage = one 128-byte swizzle row
 constexpr int kStep = 32;    // K of one kind::f8f6f4 instruction
@@ -760,13 +761,9 @@ int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, 
 
 }  // namespace
 
-int take_product_status(int *value) {
-    KREA2_CUDA(cudaMemcpyFromSymbol(value, g_product_status, sizeof(int)));
-    if (*value != 0) {
-        const int zero = 0;
-        KREA2_CUDA(cudaMemcpyToSymbol(g_product_status, &zero, sizeof(int)));
-    }
-    return KREA2_OK;
+int take_product_status(int mask, int *value) {
+    *value = 0;
+    return g_product_launched.load(std::memory_order_relaxed) ? take_status_bits(g_product_status, mask, value) : KREA2_OK;
 }
 
 }  // namespace krea2
@@ -793,5 +790,6 @@ extern "C" int krea2_gemm_fp8_128(krea2_stream stream, size_t m, const void *a, 
                            static_cast<uint32_t>((k_size + kBlock - 1) / kBlock), c_stride, kind == KREA2_BF16 ? 1u : 0u,
                            aligned16(c) && c_stride % 8 == 0 ? 1u : 0u, 0u};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    g_product_launched.store(true, std::memory_order_relaxed);
     return launch_product(s, a, w, k_size, a_stride, w_stride, g);
 }

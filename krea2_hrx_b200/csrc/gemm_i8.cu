@@ -1461,20 +1461,27 @@ extern "C" int krea2_shard_wait(krea2_stream stream, const uint32_t *flags, uint
     return KREA2_OK;
 }
 
-extern "C" int krea2_device_status(int *host_status) {
+extern "C" int krea2_device_status_of(int mask, int *host_status) {
     clear_error();
     KREA2_REQUIRE(host_status, "device_status: null output");
     KREA2_CUDA(cudaDeviceSynchronize());
-    int value = 0;
-    KREA2_CUDA(cudaMemcpyFromSymbol(&value, g_device_status, sizeof(int)));
-    if (value != 0) {
-        int zero = 0;
-        KREA2_CUDA(cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)));
+    int value = 0, share = 0;
+    if (mask & (KREA2_STATUS_GEMM_I8 | KREA2_STATUS_SHARD_WAIT))
+        if (int status = take_status_bits(g_device_status, mask, &value)) return status;
+    if (mask & KREA2_STATUS_ATTENTION) {
+        if (int status = take_attention_status(mask, &share)) return status;
+        value |= share;
     }
-    int attention = 0, product = 0, cross = 0;
-    if (int status = take_attention_status(&attention)) return status;
-    if (int status = take_product_status(&product)) return status;
-    if (int status = take_cross_status(&cross)) return status;
-    *host_status = value | attention | product | cross;
+    if (mask & KREA2_STATUS_GEMM_FP8) {
+        if (int status = take_product_status(mask, &share)) return status;
+        value |= share;
+    }
+    if (mask & KREA2_STATUS_CROSS_ATTENTION) {
+        if (int status = take_cross_status(mask, &share)) return status;
+        value |= share;
+    }
+    *host_status = value;
     return KREA2_OK;
 }
+
+extern "C" int krea2_device_status(int *host_status) { return krea2_device_status_of(~0, host_status); }

@@ -158,10 +158,11 @@ class SymmetricFabric:
 
 
 def require_clean_status() -> None:
-    """Reads the device status word (which synchronises the device) and raises `Runtime` when a bounded wait of a
-    sharded chain ran out, i.e. when the forward went on without a peer's data."""
-    from ._lib import Runtime, device_status
-    status = device_status()
+    """Reads the chain's bits of the device status word (which synchronises the device) and raises `Runtime` when a
+    bounded wait of a sharded chain ran out, i.e. when the forward went on without a peer's data.  What other kernels
+    of the process have raised is not the chain's, and stays for whoever launched them."""
+    from ._lib import STATUS_CHAIN, Runtime, device_status
+    status = device_status(STATUS_CHAIN)
     if status != 0:
         raise Runtime(f"device status {status}: a bounded wait of the sharded chain ran out (bit 16: a peer's data "
                       "never arrived); the result is not valid")
