@@ -324,6 +324,9 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSoftmaxRegisters));
         const uint32_t lane_bits = static_cast<uint32_t>(warp * 32) << 16;
         const uint32_t s_at = tmem + lane_bits, o_at = tmem + kRows + lane_bits;
+        // Rows past the tile's queries belong to nobody and hold what an earlier CTA left in shared memory: they have no say in
+        // whether the warp rescales O (a NaN there would have it do so for every tile).
+        const bool owned = static_cast<uint32_t>(warp * 32 + lane) < rows;
         for (uint32_t i = 0; i < count; i++) {
             uint32_t word[4];
             const uint32_t key0 = (first + i) * kRows;
@@ -362,7 +365,7 @@ cross_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             // The exponents' reference moves only when the maximum has grown by more than 2^8 (a weight of 256 is exact
             // enough in either type, and neither O nor the sum changes its ratio); NaN and infinity make the row NaN for good.
             float alpha = 1.0f;
-            const bool move = !(top <= reference + 8.0f);
+            const bool move = owned && !(top <= reference + 8.0f);
             if (move) {
                 const float next = top < INFINITY ? top : NAN;
                 alpha = exp2_approx(reference - next);
