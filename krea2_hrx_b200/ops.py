@@ -495,4 +495,4 @@ def cross_attention(q, k, v, out, kv_lengths=None, key_mask=None, scale=None, st
         mask_stride, mask_ptr = _rows(name, "key_mask", key_mask, (batch, kv_len), key_mask.dtype, device, kv_len), key_mask.data_ptr()
     _run_on(name, device, stream, lib().krea2_cross_attention, batch, q_len, kv_len, q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths_ptr, mask_ptr,
             out.data_ptr(), q_heads, kv_heads, head_dim, *q_strides, *k_strides, *v_strides, *out_strides, mask_stride,
-            head_dim ** -0.5 if scale is None else scale, kind)
+            max(1, head_dim) ** -0.5 if scale is None else scale, kind)
