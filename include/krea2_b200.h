@@ -357,7 +357,7 @@ int krea2_rotary_frequencies(size_t rotary_dim, double base, int scaling, double
  * included, changes nothing, and a row without a counting key is written as zeros.  q, out [batch][q_len][q_heads *
  * head_dim], k, v [batch][kv_len][kv_heads * head_dim] at 16-byte aligned rows (strides multiples of 8); a batch stride
  * of 0 (of q, k, v or the mask) shares one item with the whole batch.  head_dim a multiple of 8 up to 128, at most 128
- * query heads to a key head; kv_len may be 0; scale > 0. */
+ * query heads to a key head; kv_len may be 0; 0 < scale < 2^127. */
 int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q_len, size_t kv_len, const void *q, const void *k,
                           const void *v, const int32_t *kv_lengths, const void *key_mask, void *out, size_t q_heads,
                           size_t kv_heads, size_t head_dim, size_t q_batch_stride, size_t q_stride,

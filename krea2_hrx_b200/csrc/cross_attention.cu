@@ -611,7 +611,8 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
                       (out_batch_stride >= q_heads * head_dim && out_stride >= (batch - 1) * out_batch_stride + q_heads * head_dim),
                   "%s: the batch's outputs overlap", name);
     KREA2_REQUIRE(!key_mask || batch == 1 || mask_stride == 0 || mask_stride >= kv_len, "%s: mask_stride %zu is below kv_len %zu", name, mask_stride, kv_len);
-    KREA2_REQUIRE(std::isfinite(scale) && scale > 0.0f, "%s: scale must be a positive number", name);
+    const float scale_log2 = scale * 1.44269504088896340736f;  // infinite for the largest scales, which would make zero scores NaN
+    KREA2_REQUIRE(std::isfinite(scale_log2) && scale > 0.0f, "%s: scale must be a positive number below 2^127", name);
     KREA2_REQUIRE(kind == KREA2_F16 || kind == KREA2_BF16, "%s: kind %d is neither KREA2_F16 nor KREA2_BF16", name, kind);
     KREA2_REQUIRE(q && out && (kv_len == 0 || (k && v)), "%s: null buffer", name);
     KREA2_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "%s: buffers must be 16-byte aligned", name);
@@ -623,7 +624,7 @@ extern "C" int krea2_cross_attention(krea2_stream stream, size_t batch, size_t q
                v_shared = batch > 1 && v_batch_stride == 0;
     const CrossArgs g = {kv_lengths, static_cast<const uint8_t *>(key_mask), static_cast<uint16_t *>(out), static_cast<uint32_t>(q_len),
                          static_cast<uint32_t>(kv_len), h, queries, static_cast<uint32_t>(head_dim), out_batch_stride, out_stride, mask_stride,
-                         q_shared ? 1u : 0u, k_shared ? 1u : 0u, v_shared ? 1u : 0u, scale * 1.44269504088896340736f};
+                         q_shared ? 1u : 0u, k_shared ? 1u : 0u, v_shared ? 1u : 0u, scale_log2};
     CrossMaps maps = {};  // without keys none is loaded
     if (int status = states_map(&maps.q, bf16, q, head_dim, q_heads, q_len, q_shared ? 1 : batch, q_stride, q_batch_stride, h, queries)) return status;
     if (int status = states_map(&maps.out, bf16, out, head_dim, q_heads, q_len, batch, out_stride, out_batch_stride, h, queries)) return status;
