@@ -328,7 +328,8 @@ int krea2_prepare_plain_fp8(krea2_stream stream, size_t tokens, const void *x, v
 /* c[i][j] = kind(sum over blocks g of 128 channels: a_scale[i][g] * scale[j/128][g] * sum of a[i][k] * w[j][k] in g).
  * a e4m3 [m][a_stride], w e4m3 [n_size][w_stride], both K-contiguous; a_scale f32 [m][ceil(k_size/128)], scale f32
  * [ceil(n_size/128)][ceil(k_size/128)].  Any m, n_size and k_size (up to 2^24, 262144, 65536); a_stride and w_stride
- * multiples of 16, codes beyond k_size are never used. */
+ * multiples of 16, codes beyond k_size are never used.  The two scales are multiplied in f32 first, so their product has to
+ * lie in its range: beyond 2^128 it is infinite, below 2^-126 it loses bits. */
 int krea2_gemm_fp8_128(krea2_stream stream, size_t m, const void *a, const void *w, const float *scale,
                        const float *a_scale, void *c, size_t k_size, size_t a_stride, size_t w_stride, size_t n_size,
                        size_t c_stride, int kind);

@@ -15,7 +15,7 @@
 // Bound by the chain of a row tile, scores -> softmax -> second product, of which an SM has two under way: 16384 queries of
 // 48/12 heads of 128 to 512 keys take 240-265 us (0.78-0.86 PFLOP/s: four key tiles a CTA, so its start and end weigh), 4608
 // to 4608 480 us (1.09 PFLOP/s, tensor pipe 0.5 active).  Heads of 64 do half the products for the same exponentials and are
-// bound by those; a mask's selects cost 22-30 % more softmax.  One row tile per head of a single query: 7.3 us for 512 keys.
+// bound by those; a mask's selects cost 22-30 % more softmax.  One row tile per head of a single query: 7.3-10 us for 512 keys.
 // Where the rows do not fill the device, a cluster of up to eight CTAs splits the keys of a row tile and adds its partial
 // outputs over distributed shared memory in the order of their rank: no workspace, the same bits every time.
 #include <atomic>
@@ -32,7 +32,9 @@ constexpr int kCrossTimedOut = KREA2_STATUS_CROSS_ATTENTION;
 
 constexpr int kRows = 128;  // query rows of a CTA, keys of a tile
 
-// Weights are rounded to the tensors' type for the second product (half a step each; their sum is taken before).  A weight
+// Weights are rounded to the tensors' type for the second product (half a step each; their sum is taken before), as the tensor
+// cores need them: the error of an output against 64 bits is 1.2-1.4 times that of weights in f32 (bf16 0.0021-0.0023 against
+// 0.0017 of it, f16 0.00026-0.00029 against 0.00021).  A weight
 // far below its row's largest would be lost in f16, whose numbers end at 2^-25, and many such may count, so f16 weights
 // carry a factor of 2^7, which drops out with the sum: the largest is 2^15 (the reference lags by 2^8 at most), and what is
 // 2^-32 of the reference still counts.

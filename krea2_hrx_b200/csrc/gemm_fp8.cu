@@ -115,11 +115,13 @@ struct ScaleRing {
 };
 
 // ---------------------------------------------------------------- wide
-// Bound by what the block scales cost: a block's four products take 512 clocks of the pair's tensor cores, but its 256 x 256
-// sums also leave tensor memory and pass through the FMA pipes each time, and the two get in each other's way: 735 clocks a
-// block.  4608 x 15360 x 6144 takes 409-445 us (2.0-2.1 PFLOP/s, 0.6 of the e4m3 rate; 1.5 GHz at the power cap).  With an
-// eighth of the sums read it took 341 us, with a quarter of the products 346, with both 228.  Sixteen epilogue warps, loads
-// of 32 columns, one product of 256 columns instead of two of 128: no faster.
+// Bound by what the block scales cost and by the ends of a tile.  A block's four products take 512 clocks of the pair's tensor
+// cores, but its 256 x 256 sums also leave tensor memory and pass through the FMA pipes each time: 782 clocks a block.  A tile's
+// output holds back the next one's sums, of which two blocks at most are computed ahead: 5200 clocks a tile.  (Both from the
+// time times the sampled SM clock of 4608 x 15360 at 1024 to 10240 channels, 15 rounds of tiles.)  4608 x 15360 x 6144 takes
+// 380-445 us (2.0-2.3 PFLOP/s, 0.6-0.7 of the e4m3 rate; 441 us at 1432 MHz, back to back at the power cap).  With an eighth
+// of the sums read it took 341 us, with a quarter of the products 346, with both 228, each at the clock that the cap left it.
+// Sixteen epilogue warps, loads of 32 columns, one product of 256 columns instead of two of 128: no faster.
 struct Wide {
     static constexpr int kRows = 128;     // of a, and of w, per CTA
     static constexpr int kColumns = 256;  // of a tile
@@ -396,7 +398,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 }
 
 // ---------------------------------------------------------------- narrow
-// One row: bound by HBM once the weights are large (15360 x 16384: 50 us, 5.05 TB/s), by the start, the ramp of the loads and
+// One row: bound by HBM once the weights are large (15360 x 16384: 46 us, 5.5 TB/s), by the start, the ramp of the loads and
 // the addition of the shares below (6144 x 6144: 11.2 us against 5.9 for the bytes).  A few hundred rows: by what the tiles
 // take out of L2, 13-15 TB/s (275 x 6144 x 16384: 43 us).
 constexpr int power_of_two(int n) { return n <= 32 ? 32 : 2 * power_of_two((n + 1) / 2); }
@@ -718,7 +720,11 @@ int launch_wide(cudaStream_t stream, const void *a, const void *w, size_t k, siz
 // The kernel and tile that are expected to take least.  The wide kernel takes 7.5 us and, for each round of tiles over the
 // pairs of SMs, 1 us and 0.4 us a block.  It has the rows that fill its tiles: of 6144 columns and channels it takes 26 us for
 // 128 to 512 rows and 29 for 768, the narrow one (its best tile) 16 for 64, 17 for 128, 20 for 192, 26 for 384, 32 for 512
-// and 47 for 768.  Beyond 1024 rows no shape's estimate chooses the narrow one.
+// and 47 for 768.  Beyond 1024 rows the wide kernel is taken without an estimate.  That is right where its tiles fill the pairs
+// (1043 x 6144 x 6144 48.6 us, narrow 59.6; 2048 x 1536 x 6144 25.3 and 30.4; 4608 x 1536 x 6144 47.3 and 59.8).  It costs
+// few columns, which leave most pairs idle and whose channels it does not split: 1043 x 1536 x 6144 24.4 us, narrow 19.0;
+// 1043 x 1536 x 16384 55.1 and 36.1; 4608 x 256 x 6144 25.0 and 16.4; 2048 x 256 x 16384 55.2 and 20.5; 1025 x 128 x 16384
+// 54.1 and 11.4.
 int launch_product(cudaStream_t stream, const void *a, const void *w, size_t k, size_t a_stride, size_t w_stride, const ProductArgs &g) {
     NarrowPlan plan;
 #define KREA2_NARROW(tokens)                                                                       \

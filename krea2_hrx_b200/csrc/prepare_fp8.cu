@@ -275,10 +275,12 @@ int launch_runs(cudaStream_t stream, const PrepareArgs &g, uint32_t runs) {
     return KREA2_OK;
 }
 
-// Few rows (or narrow ones): one run a thread, for the latency (2.8 us for one row of 6144).  Many: two or three, so that
+// Few rows (or narrow ones): one run a thread, for the latency (2.7 us for one row of 6144).  Many: two or three, so that
 // four blocks of up to 256 threads share an SM and one's loads run under another's sums: 4608 rows of 6144 and their
-// residual take 38 us (80 % of the HBM rate, 89 % for 16896 rows), 70 us with one run a thread and a block per row.  Wider
+// residual take 38 us (82 % of the HBM rate, 91 % for 16896 rows), 70 us with one run a thread and a block per row.  Wider
 // rows: two runs in up to 1024 threads, 28 us for 1043 rows of 16384 and their residual, 32 us with four runs in 512.
+// Narrow rows have a block of one warp, of which an SM holds 32: 110592 rows of 256 and their residual take 37 us (83 %),
+// 221184 rows of 128, where half of the lanes idle, 69 us (45 %).
 template <bool kBf16, bool kNorm, bool kResidual, bool kVector>
 int launch_prepare(cudaStream_t stream, const PrepareArgs &g) {
     const uint32_t runs = (g.width + 7) / 8;

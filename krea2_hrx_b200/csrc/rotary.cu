@@ -41,10 +41,11 @@ __device__ __forceinline__ float low_value(uint32_t word) { return value_of<kBf1
 template <bool kBf16>
 __device__ __forceinline__ float high_value(uint32_t word) { return value_of<kBf16>(static_cast<uint16_t>(word >> 16)); }
 
-// HBM-bound: 4608 tokens of 48 + 12 heads of 128 take 26.4 us (5.4 TB/s of reads and writes, 0.83 of the copy rate), 55 us
-// with a lane per pair and element-wise accesses; one token 2.6 us.  A warp walks heads of one token, four heads' loads in flight (the first are under way before the angles are
-// taken); `warps` warps share a token's heads where the tokens do not fill the device.  The token's cosines and sines are
-// taken once per warp, a pair per lane, and lie in shared memory; a lane keeps those of its piece in registers.
+// HBM-bound: 4608 tokens of 48 + 12 heads of 128 take 26.4-28.1 us (5.0-5.4 TB/s of reads and writes, 0.78-0.83 of the copy
+// rate), 55 us with a lane per pair and element-wise accesses; one token 2.6-3.6 us.  A warp walks heads of one token, four
+// heads' loads in flight (the first are under way before the angles are taken); `warps` warps share a token's heads where the
+// tokens do not fill the device.  The token's cosines and sines are taken once per warp, a pair per lane, and lie in shared
+// memory; a lane keeps those of its piece in registers.
 constexpr int kBatch = 4;
 
 __device__ __forceinline__ void take_turns(const RotaryArgs &g, size_t token, uint32_t lane, float2 *turn) {
